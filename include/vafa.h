@@ -44,7 +44,7 @@ enum vafa_error {
 typedef void* vafa_stream_t; /* a cudaStream_t */
 
 /* Status word layout (4 x int32 in device memory, caller-zeroed once; kernels only ever
- * write non-zero codes): [0] error code (0 = none), [1] kernel/site id, [2] detail (e.g. the
+ * write non-zero codes): [0] error code (0 = none; 4: a length, position or page id outside its array), [1] kernel/site id, [2] detail (e.g. the
  * work item), [3] reserved.  vafa_check_status() reads it after the caller has synchronised. */
 #define VAFA_STATUS_WORDS 4
 
@@ -206,6 +206,81 @@ int vafa_absorb_inner_bwd(const vafa_absorb_args* a, vafa_stream_t stream);
  * gradients have been summed across ranks.  Replaces the torch casts at
  * triton_target_attn_absorb/triton_target_attn_absorb/interface.py:318-319. */
 int vafa_cast_from_f32(const float* src, void* dst, size_t n, int32_t dtype, vafa_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Positions and serving: rotation of packed queries and keys, a paged key/value cache, attention of new
+ * tokens over it.  No counterpart in the reference, which has neither positions nor a cache.
+ *
+ * A cache is two arrays of pages, element (page, slot, head, d) at page * page_stride + slot * slot_stride +
+ * head * head_stride + d (elements; the three strides of each array are free, so that K and V may be halves of one
+ * array and heads may come before slots).  Token j of sequence s lies in slot j % page_size of page
+ * page_table[s * table_stride + j / page_size].  Lengths, page ids and positions are read on the device: one that leaves its
+ * array is not followed, and code 4 goes to the status word.
+ * ------------------------------------------------------------------------------------- */
+typedef struct vafa_rotary_args {
+  const void* q;        /* [total, H, D], strides below; NULL with num_heads 0 */
+  const void* k;        /* [total, H_kv, D]; NULL with num_kv_heads 0 */
+  void* q_out;          /* contiguous */
+  void* k_out;
+  const float* cos;     /* [table_rows, rotary_dim / 2] fp32, contiguous */
+  const float* sin;
+  const int32_t* positions;   /* [total], or NULL: a token's place in its segment of cu_seqlens */
+  const int32_t* cu_seqlens;  /* [n_seg + 1]; rows behind the last segment come out as zeros */
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride; /* elements; the last dim is contiguous */
+  int32_t n_seg, total, num_heads, num_kv_heads, head_dim, rotary_dim, table_rows, dtype;
+  int32_t interleaved;  /* 0: pairs (i, i + R/2), 1: pairs (2i, 2i + 1) */
+  int32_t inverse;      /* 1: rotate back, which is the gradient */
+  int32_t* status;
+} vafa_rotary_args;
+
+/* A token whose position is outside the table comes out as NaN. */
+int vafa_rotary(const vafa_rotary_args* a, vafa_stream_t stream);
+
+typedef struct vafa_paged_append_args {
+  const void* q;        /* [total, H, D] or NULL: queries to be rotated beside */
+  const void* k;        /* [total, H_kv, D]: new keys, rotated on the way when cos is given */
+  const void* v;        /* [total, H_kv, D] */
+  void* q_out;          /* [total, H, D] contiguous */
+  void* k_cache;
+  void* v_cache;
+  const float* cos;     /* [table_rows, rotary_dim / 2], or NULL: no rotation (q must be NULL then) */
+  const float* sin;
+  const int32_t* cu_seqlens;    /* [n_seq + 1]: new tokens of each sequence, or NULL: one each (total = n_seq) */
+  const int32_t* cache_seqlens; /* [n_seq]: tokens of each sequence, the new ones among them; 0: a padding sequence,
+                                   whose new tokens are passed over */
+  const int32_t* page_table;    /* [n_seq, max_pages] */
+  int64_t q_token_stride, q_head_stride, k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+  int64_t k_page_stride, k_slot_stride, k_cache_head_stride, v_page_stride, v_slot_stride, v_cache_head_stride;
+  int64_t table_stride;
+  int32_t n_seq, total, num_heads, num_kv_heads, head_dim, rotary_dim, table_rows, num_pages, page_size, max_pages, dtype;
+  int32_t interleaved;
+  int32_t* status;
+} vafa_paged_append_args;
+
+int vafa_paged_append(const vafa_paged_append_args* a, vafa_stream_t stream);
+
+typedef struct vafa_paged_attn_args {
+  const void* q;        /* [n_seq, q_len, H, D]; strides below */
+  const void* k_cache;
+  const void* v_cache;
+  void* o;              /* [n_seq, q_len, H, D] contiguous */
+  float* lse;           /* [n_seq, q_len, H] natural log, or NULL */
+  const int32_t* cache_seqlens; /* [n_seq], the q_len new tokens among them: token t of sequence s sees the keys
+                                   j <= cache_seqlens[s] - q_len + t.  A row that sees none gives o = 0, lse = -inf */
+  const int32_t* page_table;
+  int64_t q_seq_stride, q_token_stride, q_head_stride;
+  int64_t k_page_stride, k_slot_stride, k_cache_head_stride, v_page_stride, v_slot_stride, v_cache_head_stride;
+  int64_t table_stride;
+  int32_t n_seq, q_len, num_heads, num_kv_heads, head_dim, num_pages, page_size, max_pages, dtype;
+  float scale;
+  int32_t sm_count;     /* 0: query the current device */
+  void* workspace;      /* >= vafa_paged_decode_workspace_bytes(), 256-byte aligned */
+  size_t workspace_bytes;
+  int32_t* status;
+} vafa_paged_attn_args;
+
+size_t vafa_paged_decode_workspace_bytes(const vafa_paged_attn_args* a);
+int vafa_paged_decode(const vafa_paged_attn_args* a, vafa_stream_t stream);
 
 /* ---- housekeeping ------------------------------------------------------------------ */
 /* A check on the host of two prefix-sum arrays of n_seg + 1 entries on the device: both start at 0, end at their

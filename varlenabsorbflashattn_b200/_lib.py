@@ -32,6 +32,7 @@ EXPORTS = (
     "vafa_absorb_fwd", "vafa_absorb_bwd", "vafa_absorb_bwd_phase", "vafa_absorb_inner_fwd", "vafa_absorb_inner_bwd",
     "vafa_profile_enable", "vafa_profile_kernel_count", "vafa_profile_kernel_name", "vafa_profile_read",
     "vafa_profile_reset", "vafa_set_wait_limit_cycles", "vafa_selftest_bounded_wait", "vafa_set_varlen_bwd_mode",
+    "vafa_rotary", "vafa_paged_append", "vafa_paged_decode", "vafa_paged_decode_workspace_bytes",
 )
 
 
@@ -60,6 +61,34 @@ class AbsorbArgs(C.Structure):
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
         ("x_width", C.c_int32),
     ]
+
+
+def _fields(pointers="", longs="", ints="", more=()):
+    return ([(n, C.c_void_p) for n in pointers.split()] + [(n, C.c_int64) for n in longs.split()]
+            + [(n, C.c_int32) for n in ints.split()] + list(more))
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = _fields("q k q_out k_out cos sin positions cu_seqlens", "q_token_stride q_head_stride k_token_stride k_head_stride",
+                       "n_seg total num_heads num_kv_heads head_dim rotary_dim table_rows dtype interleaved inverse",
+                       [("status", C.c_void_p)])
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = _fields("q k v q_out k_cache v_cache cos sin cu_seqlens cache_seqlens page_table",
+                       "q_token_stride q_head_stride k_token_stride k_head_stride v_token_stride v_head_stride k_page_stride k_slot_stride "
+                       "k_cache_head_stride v_page_stride v_slot_stride v_cache_head_stride table_stride",
+                       "n_seq total num_heads num_kv_heads head_dim rotary_dim table_rows num_pages page_size max_pages dtype interleaved",
+                       [("status", C.c_void_p)])
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = _fields("q k_cache v_cache o lse cache_seqlens page_table",
+                       "q_seq_stride q_token_stride q_head_stride k_page_stride k_slot_stride k_cache_head_stride v_page_stride v_slot_stride "
+                       "v_cache_head_stride table_stride",
+                       "n_seq q_len num_heads num_kv_heads head_dim num_pages page_size max_pages dtype",
+                       [("scale", C.c_float), ("sm_count", C.c_int32), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+                        ("status", C.c_void_p)])
 
 
 _lib = None
@@ -105,6 +134,11 @@ def load() -> C.CDLL:
                      "vafa_absorb_fwd_checked", "vafa_absorb_inner_fwd_checked"):
             getattr(lib, name).argtypes = [C.POINTER(AbsorbArgs), C.c_void_p]
             getattr(lib, name).restype = C.c_int
+        for name, args in (("vafa_rotary", RotaryArgs), ("vafa_paged_append", PagedAppendArgs), ("vafa_paged_decode", PagedAttnArgs)):
+            getattr(lib, name).argtypes = [C.POINTER(args), C.c_void_p]
+            getattr(lib, name).restype = C.c_int
+        lib.vafa_paged_decode_workspace_bytes.argtypes = [C.POINTER(PagedAttnArgs)]
+        lib.vafa_paged_decode_workspace_bytes.restype = C.c_size_t
         lib.vafa_absorb_bwd_phase.argtypes = [C.POINTER(AbsorbArgs), C.c_int32, C.c_void_p]
         lib.vafa_absorb_bwd_phase.restype = C.c_int
         lib.vafa_set_varlen_bwd_mode.argtypes = [C.c_int]

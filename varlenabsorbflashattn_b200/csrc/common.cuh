@@ -39,7 +39,7 @@ int varlen_bwd_mode();
 
 // ---- device-side status word ----------------------------------------------------------
 // Kernels report failures (a wait that ran out, a bad work item) by writing a non-zero code
-// once; they never trap.  Codes: 1 = mbarrier wait ran out, 2 = bad work item, 3 = TMEM.
+// once; they never trap.  Codes: 1 = mbarrier wait ran out, 2 = bad work item, 3 = TMEM, 4 = index out of range.
 __device__ __forceinline__ void report_error(int32_t* status, int code, int site, int detail) {
   if (status != nullptr) {
     if (atomicCAS(status, 0, code) == 0) {

@@ -1,0 +1,165 @@
+// C ABI of the rotation, the paged append and the paged decode: argument checks and the choice of a decode tile.
+#include <string.h>
+
+#include "paged_decode.cuh"
+
+namespace vafa {
+namespace {
+
+bool dtype_ok(int d) { return d == VAFA_F32 || d == VAFA_BF16 || d == VAFA_F16; }
+bool dim_ok(int d) { return d == 16 || d == 32 || d == 64 || d == 128 || d == 256; }
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+int check_table(const float* cos, const float* sin, int R, int D, int rows) {
+  if (!cos || !sin) return fail(VAFA_ERR_INVALID, "null cos/sin");
+  if (!aligned(cos, 4) || !aligned(sin, 4)) return fail(VAFA_ERR_INVALID, "cos/sin must be 4-byte aligned");
+  if (R < 2 || R > D || (R & 1)) return fail(VAFA_ERR_INVALID, "rotary_dim %d must be even, 2 to head_dim %d", R, D);
+  if (rows < 0) return fail(VAFA_ERR_INVALID, "bad table_rows %d", rows);
+  return 0;
+}
+
+int check_cache(const void* k, const void* v, const int32_t* lens, const int32_t* table, int n_seq, int pages, int page_size, int max_pages) {
+  if (!k || !v) return fail(VAFA_ERR_INVALID, "null cache");
+  if (!lens || !table) return fail(VAFA_ERR_INVALID, "null cache_seqlens/page_table");
+  if (n_seq < 1 || pages < 1 || page_size < 1 || max_pages < 1)
+    return fail(VAFA_ERR_INVALID, "bad sizes n_seq=%d num_pages=%d page_size=%d max_pages=%d", n_seq, pages, page_size, max_pages);
+  if ((long long)max_pages * page_size > 0x7fffffffLL - 65536)
+    return fail(VAFA_ERR_INVALID, "max_pages %d x page_size %d exceeds int32 range", max_pages, page_size);
+  return 0;
+}
+
+int check_decode(const vafa_paged_attn_args* a) {
+  if (!a) return fail(VAFA_ERR_INVALID, "null args");
+  if (!dtype_ok(a->dtype)) return fail(VAFA_ERR_INVALID, "bad dtype %d", a->dtype);
+  if (!dim_ok(a->head_dim)) return fail(VAFA_ERR_UNSUPPORTED, "head_dim %d not supported (16/32/64/128/256)", a->head_dim);
+  if (a->q_len < 1 || a->num_heads < 1 || a->num_kv_heads < 1 || a->num_heads % a->num_kv_heads)
+    return fail(VAFA_ERR_INVALID, "bad sizes q_len=%d H=%d H_kv=%d (H_kv must divide H)", a->q_len, a->num_heads, a->num_kv_heads);
+  if ((long long)a->q_len * a->num_heads > (1 << 20)) return fail(VAFA_ERR_UNSUPPORTED, "q_len %d x %d heads", a->q_len, a->num_heads);
+  if (const int rc = check_cache(a->k_cache, a->v_cache, a->cache_seqlens, a->page_table, a->n_seq, a->num_pages, a->page_size, a->max_pages)) return rc;
+  return 0;
+}
+
+paged::Plan plan_for(const vafa_paged_attn_args* a) {
+  const int R = a->q_len * (a->num_heads / a->num_kv_heads);
+  return a->dtype == VAFA_F32 ? paged::plan_f32(a->head_dim, R) : a->dtype == VAFA_BF16 ? paged::plan_bf16(a->head_dim, R) : paged::plan_f16(a->head_dim, R);
+}
+
+// CTAs of a call, and whether a unit can end up in several of them: from the room that the page table has, as the lengths are on the device.
+struct Cut {
+  int ctas, min_share;
+  bool splits;
+  size_t part_o, part_ml, meta;
+};
+
+int cut_for(const vafa_paged_attn_args* a, const paged::Plan& plan, Cut* c) {
+  int sms = a->sm_count;
+  if (sms <= 0) {
+    int dev = 0;
+    VAFA_CUDA_CHECK(cudaGetDevice(&dev));
+    VAFA_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+  }
+  const long long per_unit = ((long long)a->max_pages * a->page_size + plan.bk - 1) / plan.bk;
+  const long long per_seq = (long long)a->num_kv_heads * plan.row_tiles * per_unit;
+  if (per_seq > 0x7fffffffLL) return fail(VAFA_ERR_UNSUPPORTED, "a sequence has too many heads and keys");
+  const long long most = per_seq * a->n_seq;
+  c->min_share = 2;
+  const long long want = (most + c->min_share - 1) / c->min_share;
+  c->ctas = (int)(want < (long long)sms * plan.ctas_per_sm ? want : (long long)sms * plan.ctas_per_sm);
+  c->splits = per_unit > 1;
+  c->part_o = align_up((size_t)2 * c->ctas * plan.rows * a->head_dim * 4, 256);
+  c->part_ml = align_up((size_t)2 * c->ctas * plan.rows * 8, 256);
+  c->meta = align_up((size_t)c->ctas * 16, 256);
+  return 0;
+}
+
+}  // namespace
+
+size_t paged_decode_workspace(const vafa_paged_attn_args* a) {
+  Cut c;
+  if (cut_for(a, plan_for(a), &c)) return 0;
+  return c.part_o + c.part_ml + c.meta;
+}
+
+int paged_decode_launch(const vafa_paged_attn_args* a, cudaStream_t s) {
+  const paged::Plan plan = plan_for(a);
+  Cut c;
+  if (const int rc = cut_for(a, plan, &c)) return rc;
+  const size_t need = c.part_o + c.part_ml + c.meta;
+  if (!a->workspace || a->workspace_bytes < need) return fail(VAFA_ERR_WORKSPACE, "workspace too small: have %zu, need %zu", a->workspace_bytes, need);
+  if (!aligned(a->workspace, 256)) return fail(VAFA_ERR_WORKSPACE, "workspace must be 256-byte aligned");
+  paged::DecodeParams p;
+  memset(&p, 0, sizeof(p));
+  p.q = a->q; p.k = a->k_cache; p.v = a->v_cache; p.o = a->o; p.lse = a->lse;
+  p.lens = a->cache_seqlens; p.table = a->page_table;
+  p.q_seq = a->q_seq_stride; p.q_token = a->q_token_stride; p.q_head = a->q_head_stride;
+  p.k_page = a->k_page_stride; p.k_slot = a->k_slot_stride; p.k_head = a->k_cache_head_stride;
+  p.v_page = a->v_page_stride; p.v_slot = a->v_slot_stride; p.v_head = a->v_cache_head_stride;
+  p.table_stride = a->table_stride;
+  p.n_seq = a->n_seq; p.T = a->q_len; p.H = a->num_heads; p.H_kv = a->num_kv_heads;
+  p.g = a->num_heads / a->num_kv_heads; p.R = p.T * p.g;
+  p.row_tiles = plan.row_tiles; p.num_pages = a->num_pages; p.page_size = a->page_size;
+  p.capacity = a->max_pages * a->page_size;
+  p.scale_log2 = a->scale * kLog2e;
+  char* ws = (char*)a->workspace;
+  p.part_o = (float*)ws;
+  p.part_ml = (float2*)(ws + c.part_o);
+  p.meta = (int4*)(ws + c.part_o + c.part_ml);
+  p.status = a->status;
+  return plan.launch(p, c.ctas, c.min_share, c.splits, s);
+}
+
+}  // namespace vafa
+
+using namespace vafa;
+
+extern "C" {
+#pragma GCC visibility push(default)
+
+int vafa_rotary(const vafa_rotary_args* a, vafa_stream_t stream) {
+  if (!a) return fail(VAFA_ERR_INVALID, "null args");
+  if (!dtype_ok(a->dtype)) return fail(VAFA_ERR_INVALID, "bad dtype %d", a->dtype);
+  if (!dim_ok(a->head_dim)) return fail(VAFA_ERR_UNSUPPORTED, "head_dim %d not supported (16/32/64/128/256)", a->head_dim);
+  if (a->total < 0 || a->num_heads < 0 || a->num_kv_heads < 0) return fail(VAFA_ERR_INVALID, "bad sizes");
+  if (const int rc = check_table(a->cos, a->sin, a->rotary_dim, a->head_dim, a->table_rows)) return rc;
+  if (!a->positions && (!a->cu_seqlens || a->n_seg < 1)) return fail(VAFA_ERR_INVALID, "neither positions nor cu_seqlens");
+  if (a->total > 0 && ((a->num_heads > 0 && (!a->q || !a->q_out)) || (a->num_kv_heads > 0 && (!a->k || !a->k_out))))
+    return fail(VAFA_ERR_INVALID, "null q/k");
+  return rotary_launch(a, (cudaStream_t)stream);
+}
+
+int vafa_paged_append(const vafa_paged_append_args* a, vafa_stream_t stream) {
+  if (!a) return fail(VAFA_ERR_INVALID, "null args");
+  if (!dtype_ok(a->dtype)) return fail(VAFA_ERR_INVALID, "bad dtype %d", a->dtype);
+  if (!dim_ok(a->head_dim)) return fail(VAFA_ERR_UNSUPPORTED, "head_dim %d not supported (16/32/64/128/256)", a->head_dim);
+  if (a->total < 0 || a->num_kv_heads < 1 || (a->q && a->num_heads < 1)) return fail(VAFA_ERR_INVALID, "bad sizes");
+  int rc;
+  if (a->cos || a->sin) {
+    if ((rc = check_table(a->cos, a->sin, a->rotary_dim, a->head_dim, a->table_rows))) return rc;
+  } else if (a->q) {
+    return fail(VAFA_ERR_INVALID, "q without cos/sin");
+  }
+  if ((rc = check_cache(a->k_cache, a->v_cache, a->cache_seqlens, a->page_table, a->n_seq, a->num_pages, a->page_size, a->max_pages))) return rc;
+  if (!a->cu_seqlens && a->total != a->n_seq) return fail(VAFA_ERR_INVALID, "without cu_seqlens total %d must be n_seq %d", a->total, a->n_seq);
+  if (a->total > 0 && (!a->k || !a->v || (a->q && !a->q_out))) return fail(VAFA_ERR_INVALID, "null k/v/q_out");
+  return paged_append_launch(a, (cudaStream_t)stream);
+}
+
+size_t vafa_paged_decode_workspace_bytes(const vafa_paged_attn_args* a) {
+  return check_decode(a) ? 0 : paged_decode_workspace(a);
+}
+
+int vafa_paged_decode(const vafa_paged_attn_args* a, vafa_stream_t stream) {
+  if (const int rc = check_decode(a)) return rc;
+  if (!a->q || !a->o) return fail(VAFA_ERR_INVALID, "null q/o");
+  const int es = elem_size(a->dtype);
+  auto of = [](int n, int64_t stride) { return n > 1 ? stride : 0; };  // (a dim of one element may have any stride)
+  const int64_t strides = of(a->n_seq, a->q_seq_stride) | of(a->q_len, a->q_token_stride) | of(a->num_heads, a->q_head_stride) |
+                          of(a->num_pages, a->k_page_stride | a->v_page_stride) | of(a->page_size, a->k_slot_stride | a->v_slot_stride) |
+                          of(a->num_kv_heads, a->k_cache_head_stride | a->v_cache_head_stride);
+  if (!aligned(a->q, 16) || !aligned(a->k_cache, 16) || !aligned(a->v_cache, 16) || !aligned(a->o, 16) || (strides * es) % 16)
+    return fail(VAFA_ERR_INVALID, "q, o and the caches need 16-byte aligned bases and strides");
+  return paged_decode_launch(a, (cudaStream_t)stream);
+}
+
+#pragma GCC visibility pop
+}

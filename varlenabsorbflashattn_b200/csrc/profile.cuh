@@ -26,6 +26,10 @@ enum KernelId {
   kKBwdFused,
   kKBwdDqFin,
   kKAbsorbBwdDxu,
+  kKRotary,
+  kKPagedAppend,
+  kKPagedDecode,
+  kKPagedCombine,
   kKCount
 };
 

@@ -872,7 +872,7 @@ int vafa_check_status(const int32_t* status, vafa_stream_t stream) {
   if (e == cudaSuccess) e = cudaStreamSynchronize((cudaStream_t)stream);
   if (e != cudaSuccess) return fail(VAFA_ERR_CUDA, "status read failed: %s", cudaGetErrorString(e));
   if (h[0] == 0) return 0;
-  const char* what = h[0] == 1 ? "a bounded wait ran out" : h[0] == 2 ? "bad work item" : h[0] == 3 ? "tensor memory" : "unknown";
+  const char* what = h[0] == 1 ? "a bounded wait ran out" : h[0] == 2 ? "bad work item" : h[0] == 3 ? "tensor memory" : h[0] == 4 ? "a length, position or page outside its array" : "unknown";
   return fail(VAFA_ERR_DEVICE, "device error %d (%s) at site %d, detail %d", h[0], what, h[1], h[2]);
 }
 

@@ -1,0 +1,431 @@
+"""Positions and serving: rotation of packed queries and keys, a paged key/value cache, attention of new tokens over it.
+
+The reference has no counterpart.  The calls stand around `packed_varlen_attn`: a training step or a prompt runs
+
+    q, k = packed_rotary(q, k, cos, sin, cu_seqlens=cu)
+    o = packed_varlen_attn(q, k, v, cu_seqlens_q=cu, cu_seqlens_k=cu, causal=True)
+    paged_kv_append(k, v, k_cache, v_cache, page_table=table, cache_seqlens=lens, cu_seqlens=cu)     # serving
+
+and every token after it
+
+    lens += 1
+    q = paged_kv_append(k, v, k_cache, v_cache, page_table=table, cache_seqlens=lens, q=q, cos=cos, sin=sin)
+    o = paged_decode_attn(q, k_cache, v_cache, page_table=table, cache_seqlens=lens)
+
+A cache is a pair of tensors [num_pages, page_size, H_kv, D], any strides as long as the last dim is contiguous (halves
+of one tensor, or a transposed view of [num_pages, H_kv, page_size, D]).  Token j of sequence s lies in slot
+j % page_size of page page_table[s, j // page_size].  `cache_seqlens` counts the tokens of a sequence with the new ones
+among them, in both calls; a sequence of length 0 is padding, which is neither written nor attended over.
+
+As in `packed_varlen_attn` all arithmetic happens in libvafa_b200.so.  With validation on (`set_validate_cu_seqlens`,
+the default) lengths, page ids and positions are checked on the host, which waits for the device; a serving loop
+switches it off.  Unchecked, an index that leaves its array is not followed on the device either: nothing outside the tensors is read or
+written, and the status word reports it (`_lib.check_status`).
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+from . import varlen as _varlen
+from .varlen import _SUPPORTED_HEAD_DIMS, _check_cu, _lengths_to_cu
+
+__all__ = ["rotary_table", "packed_rotary", "paged_kv_append", "paged_decode_attn", "paged_decode_attn_with_lse"]
+
+
+def _need(ok: bool, message) -> None:
+    """The assertion of the other operators, which -O does not take out: the kernels go by what it says."""
+    if not ok:
+        raise AssertionError(message())
+
+
+# ------------------------------------------------------------------------------------------------
+# arguments
+# ------------------------------------------------------------------------------------------------
+def _rows(x: torch.Tensor, name: str) -> Tuple[torch.Tensor, bool]:
+    """[T, H, D] of a packed tensor, at its own strides as long as the last dim is contiguous."""
+    was4 = x.dim() == 4
+    if was4:
+        if x.shape[0] != 1:
+            raise ValueError(f"{name}: 4-D input must have batch=1 (packed varlen), got shape {tuple(x.shape)}")
+        x = x[0]
+    elif x.dim() != 3:
+        raise ValueError(f"{name}: expected 3-D [T,H,D] or 4-D [1,T,H,D], got {x.dim()}-D")
+    return (x if x.stride(2) == 1 else x.contiguous()), was4
+
+
+def _check_heads(x: torch.Tensor, name: str) -> None:
+    _need(x.is_cuda, lambda: f"{name}: CUDA tensors are required (there is no CPU path)")
+    _need(x.dtype in _lib.DTYPE_CODE, lambda: f"{name} must be fp32, bf16 or fp16, got {x.dtype}")
+    _need(x.shape[-1] in _SUPPORTED_HEAD_DIMS, lambda: f"head_dim {x.shape[-1]} not supported (try 64/128/256)")
+
+
+def _like(x: torch.Tensor, ref: torch.Tensor, name: str) -> None:
+    _need(x.device == ref.device, lambda: f"{name}: on {x.device}, the others on {ref.device}")
+    _need(x.dtype == ref.dtype, lambda: f"{name}: dtype {x.dtype}, the others have {ref.dtype}")
+
+
+def _ints(t: torch.Tensor, device: torch.device, name: str, dims: int = 1) -> torch.Tensor:
+    """int32 on the device, the last dim contiguous."""
+    if t.dim() != dims:
+        raise ValueError(f"{name}: must be {dims}-D, got shape {tuple(t.shape)}")
+    if t.dtype is not torch.int32 or t.device != device:
+        if t.is_floating_point() or t.dtype == torch.bool:
+            raise ValueError(f"{name}: must hold integers, got {t.dtype}")
+        t = t.to(device=device, dtype=torch.int32)
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _check_angles(cos: torch.Tensor, sin: torch.Tensor, ref: torch.Tensor) -> int:
+    _need(cos.dim() == 2 and cos.shape == sin.shape, lambda: f"cos/sin must be [positions, rotary_dim/2], got {tuple(cos.shape)} and {tuple(sin.shape)}")
+    _need(cos.dtype == sin.dtype == torch.float32, lambda: f"cos/sin must be fp32, got {cos.dtype} and {sin.dtype}")
+    _need(cos.device == ref.device and sin.device == ref.device, lambda: "cos/sin must be on the device of q and k")
+    _need(cos.is_contiguous() and sin.is_contiguous(), lambda: "cos/sin must be contiguous")
+    _need(2 <= 2 * cos.shape[1] <= ref.shape[-1], lambda: f"rotary_dim {2 * cos.shape[1]} must be 2 to head_dim {ref.shape[-1]}")
+    _need(not (cos.requires_grad or sin.requires_grad), lambda: "cos/sin have no gradient here")
+    return 2 * cos.shape[1]
+
+
+def _no_gradient(what: str, *tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach its inputs")
+
+
+def _host(t: torch.Tensor) -> torch.Tensor:
+    """A copy to look over on the host (waits for the device)."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("lengths, page ids and positions cannot be checked on the host while the stream is captured: "
+                           "switch the check off (set_validate_cu_seqlens)")
+    return t.detach().to("cpu", torch.int64)
+
+
+def _check_cache(k_cache, v_cache, page_table, cache_seqlens, ref) -> None:
+    for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _need(c.dim() == 4, lambda: f"{name}: expected [num_pages, page_size, H_kv, D], got shape {tuple(c.shape)}")
+        _like(c, ref, name)
+        _need(c.stride(3) == 1, lambda: f"{name}: the last dim must be contiguous")
+    _need(k_cache.shape == v_cache.shape, lambda: f"v_cache shape {tuple(v_cache.shape)}, k_cache {tuple(k_cache.shape)}")
+    _need(k_cache.shape[3] == ref.shape[-1], lambda: f"caches have head_dim {k_cache.shape[3]}, the new tokens {ref.shape[-1]}")
+    _need(k_cache.numel() > 0, lambda: f"empty cache {tuple(k_cache.shape)}")
+    _need(page_table.shape[0] == cache_seqlens.shape[0],
+          lambda: f"page_table has {page_table.shape[0]} sequences, cache_seqlens {cache_seqlens.shape[0]}")
+    _need(page_table.shape[1] > 0 and page_table.shape[1] * k_cache.shape[1] < 2**31 - 65536,
+          lambda: f"page_table width {page_table.shape[1]} x page_size {k_cache.shape[1]} out of range")
+
+
+def _check_pages(lens: torch.Tensor, table: torch.Tensor, num_pages: int, page_size: int) -> None:
+    """Host copies: every length fits its row of the table, every page that it reaches is one of the cache's."""
+    if lens.numel() == 0:
+        return
+    if int(lens.min()) < 0 or int(lens.max()) > table.shape[1] * page_size:
+        raise ValueError(f"cache_seqlens must be 0 to {table.shape[1] * page_size} (page_table width x page_size), "
+                         f"got {int(lens.min())} to {int(lens.max())}")
+    used = torch.arange(table.shape[1])[None, :] < ((lens + page_size - 1) // page_size)[:, None]
+    if bool((used & ((table < 0) | (table >= num_pages))).any()):
+        raise ValueError(f"page_table names pages outside 0 to {num_pages - 1}")
+
+
+# ------------------------------------------------------------------------------------------------
+# rotation
+# ------------------------------------------------------------------------------------------------
+def rotary_table(positions: int, rotary_dim: int, *, base: float = 10000.0, device=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(cos, sin), fp32 [positions, rotary_dim / 2], of the angles p * base^(-2 i / rotary_dim), computed in 64 bits.
+
+    Made once and kept by the program.  The operators take any table of this shape, so other frequencies
+    (interpolated, per-band scaled) are the caller's to fill in."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if positions < 0:
+        raise ValueError(f"positions must not be negative, got {positions}")
+    w = float(base) ** (-torch.arange(0, rotary_dim, 2, dtype=torch.float64, device=device) / rotary_dim)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * w
+    return angle.cos().float(), angle.sin().float()
+
+
+def _rotate(q, k, cos, sin, positions, cu, interleaved: bool, inverse: bool):
+    ref = q if q is not None else k
+    T, D = ref.shape[0], ref.shape[2]
+    H, H_kv = (0 if x is None else x.shape[1] for x in (q, k))
+    qo = None if q is None else torch.empty((T, H, D), dtype=ref.dtype, device=ref.device)
+    ko = None if k is None else torch.empty((T, H_kv, D), dtype=ref.dtype, device=ref.device)
+    if T == 0:
+        return qo, ko
+    qs, ks = ((0, 0) if x is None else x.stride()[:2] for x in (q, k))
+    a = _lib.RotaryArgs(
+        _lib.ptr(q), _lib.ptr(k), _lib.ptr(qo), _lib.ptr(ko), cos.data_ptr(), sin.data_ptr(), _lib.ptr(positions), _lib.ptr(cu),
+        *qs, *ks, 0 if cu is None else cu.numel() - 1, T, H, H_kv, D, 2 * cos.shape[1], cos.shape[0], _lib.DTYPE_CODE[ref.dtype],
+        interleaved, inverse, _lib.status_word(ref.device).data_ptr())
+    with _lib.on_device(ref.device):
+        _lib.check(_lib.load().vafa_rotary(a, _lib.raw_stream(ref.device)), "vafa_rotary")
+        _lib.maybe_check_status(ref.device)
+    return qo, ko
+
+
+class _PackedRotary(torch.autograd.Function):
+    """y = R x per token and pair; the gradient is R^T dy, the rotation back, which has a gradient in turn."""
+
+    @staticmethod
+    def forward(ctx, q, k, cos, sin, positions, cu, interleaved, inverse):
+        ctx.save_for_backward(cos, sin, positions, cu)
+        ctx.flags = interleaved, inverse
+        ctx.set_materialize_grads(False)
+        return _rotate(q, k, cos, sin, positions, cu, interleaved, inverse)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        cos, sin, positions, cu = ctx.saved_tensors
+        interleaved, inverse = ctx.flags
+        dq = dq if dq is None or not ctx.needs_input_grad[0] or dq.stride(2) == 1 else dq.contiguous()
+        dk = dk if dk is None or not ctx.needs_input_grad[1] or dk.stride(2) == 1 else dk.contiguous()
+        dq = dq if ctx.needs_input_grad[0] else None
+        dk = dk if ctx.needs_input_grad[1] else None
+        if dq is None and dk is None:
+            return (None,) * 8
+        dq, dk = _PackedRotary.apply(dq, dk, cos, sin, positions, cu, interleaved, not inverse)
+        return dq, dk, None, None, None, None, None, None
+
+
+def packed_rotary(
+    q: torch.Tensor,
+    k: Optional[torch.Tensor],
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    *,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    seqinfo: Optional[torch.Tensor] = None,
+    positions: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """Rotate packed queries and keys by their positions, in one launch; differentiable in q and k.
+
+    q: [T, H, D] or [1, T, H, D], k: [T, H_kv, D] or [1, T, H_kv, D], or None (fp32, bf16 or fp16; D as in
+    `packed_varlen_attn`).  Tokens and heads may be strided, as in views of one projection's output.
+    cos, sin: fp32 [positions, rotary_dim / 2] (`rotary_table`).  The first rotary_dim <= D dims of a head
+    rotate, in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with `interleaved`; the others pass through.
+    A token's position is its place in its segment of cu_seqlens ([n_seg + 1]; or seqinfo: [n_seg] lengths), or
+    positions[t] where those are given ([T], any integer type).
+
+    Returns (q, k) rotated, contiguous, with the ranks of the inputs.  Rows behind the last segment, which
+    only unchecked calls can have, come out as zeros; a position outside the table gives NaN there.
+    A step with its gradients can be captured into a CUDA graph once validation is off; as with every operator, torch wants no
+    eager autograd graph of the same leaves to be alive meanwhile (its AccumulateGrad nodes belong to the eager stream).
+    """
+    q3, q4 = _rows(q, "q")
+    k3, k4 = (None, False) if k is None else _rows(k, "k")
+    _check_heads(q3, "q")
+    if k3 is not None:
+        _like(k3, q3, "k")
+        _need(k3.shape[0] == q3.shape[0] and k3.shape[2] == q3.shape[2], lambda: f"K shape mismatch: {tuple(k3.shape)} vs q {tuple(q3.shape)}")
+    _check_angles(cos, sin, q3)
+    T = q3.shape[0]
+    _lib.check_rows(T, cos.shape[0])
+    if (cu_seqlens is not None) + (seqinfo is not None) + (positions is not None) != 1:
+        raise ValueError("must provide one of cu_seqlens, seqinfo and positions")
+    if positions is None:
+        cu = _ints(cu_seqlens if seqinfo is None else _lengths_to_cu(seqinfo), q3.device, "cu_seqlens")
+        if cu.numel() < 2:
+            raise ValueError("cu_seqlens: must have at least 2 elements (n_seg+1 with n_seg>=1)")
+    else:
+        positions = _ints(positions, q3.device, "positions")
+        _need(positions.shape[0] == T, lambda: f"positions has {positions.shape[0]} entries for {T} tokens")
+        cu = None
+    if _varlen._validate and T > 0:
+        host = _host(cu if positions is None else positions)
+        if positions is None:
+            _check_cu(host, T, "cu_seqlens")
+            low, high = 0, int((host[1:] - host[:-1]).max()) - 1
+        else:
+            low, high = int(host.min()), int(host.max())
+        if low < 0 or high >= cos.shape[0]:
+            raise ValueError(f"positions {low} to {high} leave the table of {cos.shape[0]}")
+    if torch.is_grad_enabled() and (q3.requires_grad or (k3 is not None and k3.requires_grad)):
+        qo, ko = _PackedRotary.apply(q3, k3, cos, sin, positions, cu, bool(interleaved), False)
+    else:
+        qo, ko = _rotate(q3, k3, cos, sin, positions, cu, bool(interleaved), False)
+    return (qo.unsqueeze(0) if q4 else qo), (ko.unsqueeze(0) if k4 else ko)
+
+
+# ------------------------------------------------------------------------------------------------
+# append
+# ------------------------------------------------------------------------------------------------
+def _check_append(lens, table, cu, T, num_pages, page_size, angles) -> None:
+    """Host copies of an append's lengths and pages: what it would write is in the cache, and nothing twice."""
+    _check_pages(lens, table, num_pages, page_size)
+    if cu is None:
+        new = torch.ones_like(lens)
+    else:
+        _check_cu(cu, T, "cu_seqlens")
+        new = cu[1:] - cu[:-1]
+    new = torch.where(lens == 0, torch.zeros_like(new), new)  # padding
+    if bool((new > lens).any()):
+        raise ValueError("cache_seqlens must count the new tokens of a sequence among its tokens")
+    seq = torch.repeat_interleave(torch.arange(lens.numel()), new)
+    pos = torch.arange(seq.numel()) - (new.cumsum(0) - new)[seq] + (lens - new)[seq]
+    if angles is not None and pos.numel() and int(pos.max()) >= angles:
+        raise ValueError(f"position {int(pos.max())} leaves the table of {angles}")
+    slot = table[seq, pos // page_size] * page_size + pos % page_size
+    if slot.unique().numel() != slot.numel():
+        raise ValueError("page_table gives two new tokens the same slot")
+
+
+def paged_kv_append(
+    k: torch.Tensor,
+    v: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    *,
+    page_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    cu_seqlens: Optional[torch.Tensor] = None,
+    seqinfo: Optional[torch.Tensor] = None,
+    q: Optional[torch.Tensor] = None,
+    cos: Optional[torch.Tensor] = None,
+    sin: Optional[torch.Tensor] = None,
+    interleaved: bool = False,
+) -> Optional[torch.Tensor]:
+    """Write new keys and values into a paged cache, in place, rotating keys (and queries) on the way.
+
+    k, v: [T, H_kv, D] or [1, T, H_kv, D], the new tokens of all sequences; tokens and heads may be strided.
+    k_cache, v_cache: [num_pages, page_size, H_kv, D] (see the module).  page_table: [n_seq, max_pages].
+    cache_seqlens: [n_seq], tokens of each sequence with the new ones among them: new token i of the n_s of sequence
+    s goes to position cache_seqlens[s] - n_s + i.  cu_seqlens ([n_seq + 1]; or seqinfo: [n_seq]) cuts the new tokens
+    by sequence; without it there is one for each (T = n_seq).  Sequences of length 0 are padding: their tokens
+    are passed over, as are rows behind the last sequence, and so are tokens of unchecked calls whose position or page is out of range.
+    cos, sin: rotate the keys by their positions as `packed_rotary` does; q ([T, H, D]) is rotated beside them.
+    Without cos and sin keys are written as they are (rotated already).
+
+    Sequences may share pages that are only read (a common prefix); what is written must be theirs alone.
+    Returns the rotated q (contiguous; zeros for padding), or None without q.  Has no gradient.
+    """
+    k3, _ = _rows(k, "k")
+    v3, _ = _rows(v, "v")
+    _check_heads(k3, "k")
+    _like(v3, k3, "v")
+    _need(v3.shape == k3.shape, lambda: f"V shape mismatch: {tuple(v3.shape)} vs K {tuple(k3.shape)}")
+    T, H_kv, D = k3.shape
+    dev = k3.device
+    lens = _ints(cache_seqlens, dev, "cache_seqlens")
+    table = _ints(page_table, dev, "page_table", 2)
+    _check_cache(k_cache, v_cache, table, lens, k3)
+    num_pages, page_size = k_cache.shape[:2]
+    _need(k_cache.shape[2] == H_kv, lambda: f"caches have {k_cache.shape[2]} heads, k {H_kv}")
+    for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _need(all(st > 0 or n == 1 for st, n in zip(c.stride(), c.shape)), lambda: f"{name}: an expanded tensor cannot be written to")
+    _need(k_cache.data_ptr() != v_cache.data_ptr(), lambda: "k_cache and v_cache are the same memory")
+    n_seq = lens.shape[0]
+    _lib.check_rows(T, n_seq)
+    cu = None
+    if cu_seqlens is not None or seqinfo is not None:
+        cu = _ints(cu_seqlens if cu_seqlens is not None else _lengths_to_cu(seqinfo), dev, "cu_seqlens")
+        _need(cu.shape[0] == n_seq + 1, lambda: f"cu_seqlens has {cu.shape[0] - 1} sequences, cache_seqlens {n_seq}")
+    else:
+        _need(T == n_seq, lambda: f"{T} new tokens for {n_seq} sequences need cu_seqlens or seqinfo")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin go together")
+    R = rows = 0
+    if cos is not None:
+        R, rows = _check_angles(cos, sin, k3), cos.shape[0]
+    q3, q4, qo = None, False, None
+    if q is not None:
+        if cos is None:
+            raise ValueError("q is rotated by cos and sin: without them it has nothing to do here")
+        q3, q4 = _rows(q, "q")
+        _like(q3, k3, "q")
+        _need(q3.shape[0] == T and q3.shape[2] == D, lambda: f"q shape mismatch: {tuple(q3.shape)} vs K {tuple(k3.shape)}")
+        _need(q3.shape[1] > 0, lambda: "q has no heads")
+    _no_gradient("paged_kv_append", k3, v3, q3, k_cache, v_cache)
+    if q3 is not None:
+        qo = torch.empty((T, q3.shape[1], D), dtype=q3.dtype, device=dev)
+    if T > 0 and n_seq > 0:
+        if _varlen._validate:
+            _check_append(_host(lens), _host(table), None if cu is None else _host(cu), T, num_pages, page_size, rows if R else None)
+        a = _lib.PagedAppendArgs(
+            _lib.ptr(q3), k3.data_ptr(), v3.data_ptr(), _lib.ptr(qo), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(cos), _lib.ptr(sin),
+            _lib.ptr(cu), lens.data_ptr(), table.data_ptr(), *((0, 0) if q3 is None else q3.stride()[:2]), *k3.stride()[:2], *v3.stride()[:2],
+            *k_cache.stride()[:3], *v_cache.stride()[:3], table.stride(0), n_seq, T, 0 if q3 is None else q3.shape[1], H_kv, D, R, rows,
+            num_pages, page_size, table.shape[1], _lib.DTYPE_CODE[k3.dtype], bool(interleaved), _lib.status_word(dev).data_ptr())
+        with _lib.on_device(dev):
+            _lib.check(_lib.load().vafa_paged_append(a, _lib.raw_stream(dev)), "vafa_paged_append")
+            _lib.maybe_check_status(dev)
+    elif qo is not None:
+        qo.zero_()
+    return qo.unsqueeze(0) if q4 else qo
+
+
+# ------------------------------------------------------------------------------------------------
+# attention
+# ------------------------------------------------------------------------------------------------
+def _decode(q, k_cache, v_cache, page_table, cache_seqlens, scale, with_lse):
+    if q.dim() not in (3, 4):
+        raise ValueError(f"q: expected [n_seq,H,D] or [n_seq,T,H,D], got {q.dim()}-D")
+    _check_heads(q, "q")
+    dev = q.device
+    lens = _ints(cache_seqlens, dev, "cache_seqlens")
+    table = _ints(page_table, dev, "page_table", 2)
+    _check_cache(k_cache, v_cache, table, lens, q)
+    n_seq, H, D = q.shape[0], q.shape[-2], q.shape[-1]
+    T = q.shape[1] if q.dim() == 4 else 1
+    num_pages, page_size, H_kv = k_cache.shape[:3]
+    _need(n_seq == lens.shape[0], lambda: f"q has {n_seq} sequences, cache_seqlens {lens.shape[0]}")
+    _need(H % H_kv == 0, lambda: f"{H_kv} cache heads do not divide {H} query heads")
+    _no_gradient("paged_decode_attn", q, k_cache, v_cache)
+    es = q.element_size()
+    for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        if c.data_ptr() % 16 or any(n > 1 and st * es % 16 for st, n in zip(c.stride()[:3], c.shape)):
+            raise ValueError(f"{name}: base and strides must be multiples of 16 bytes")
+    if q.stride(-1) != 1 or q.data_ptr() % 16 or any(n > 1 and st * es % 16 for st, n in zip(q.stride()[:-1], q.shape)):
+        q = q.clone(memory_format=torch.contiguous_format)
+    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if with_lse else None
+    if o.numel() == 0:
+        return o, lse
+    if _varlen._validate:
+        _check_pages(_host(lens), _host(table), num_pages, page_size)
+    lib = _lib.load()
+    st = q.stride()
+    with _lib.on_device(dev):
+        a = _lib.PagedAttnArgs(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), _lib.ptr(lse), lens.data_ptr(), table.data_ptr(),
+            st[0], st[1] if q.dim() == 4 else 0, st[-2], *k_cache.stride()[:3], *v_cache.stride()[:3], table.stride(0),
+            n_seq, T, H, H_kv, D, num_pages, page_size, table.shape[1], _lib.DTYPE_CODE[q.dtype], scale, _lib.sm_count(dev),
+            None, 0, _lib.status_word(dev).data_ptr())
+        ws = _lib.workspace(lib.vafa_paged_decode_workspace_bytes(a), dev)
+        a.workspace, a.workspace_bytes = _lib.ptr(ws), 0 if ws is None else ws.numel()
+        _lib.check(lib.vafa_paged_decode(a, _lib.raw_stream(dev)), "vafa_paged_decode")
+        _lib.maybe_check_status(dev)
+    return o, lse
+
+
+def paged_decode_attn(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    *,
+    page_table: torch.Tensor,
+    cache_seqlens: torch.Tensor,
+    scale: Optional[float] = None,
+) -> torch.Tensor:
+    """Attention of the newest tokens of each sequence over its paged keys and values.
+
+    q: [n_seq, H, D], one new token for each sequence, or [n_seq, T, H, D], T of them (fp32, bf16 or fp16; D
+    as in `packed_varlen_attn`).  k_cache, v_cache: [num_pages, page_size, H_kv, D], H_kv dividing H, bases and strides
+    multiples of 16 bytes.  page_table: [n_seq, max_pages].  cache_seqlens: [n_seq], the new tokens among them: token t of sequence s sees the keys
+    j <= cache_seqlens[s] - T + t.  scale defaults to 1/sqrt(D).
+
+    Returns o with the layout of q.  A row that sees no key (a sequence of length 0, or shorter than T) yields
+    zeros.  The keys of all sequences are cut into equal pieces over the SMs whatever their lengths, and the parts
+    joined in a fixed order: the same call gives the same bits, another batch around a sequence may round
+    differently.  Meant for few new tokens; a prompt's own attention is `packed_varlen_attn`.  Has no gradient.
+    """
+    return _decode(q, k_cache, v_cache, page_table, cache_seqlens, float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1]), False)[0]
+
+
+def paged_decode_attn_with_lse(q, k_cache, v_cache, *, page_table, cache_seqlens, scale=None):
+    """As paged_decode_attn, and also returns the natural-log LSE (fp32, q's shape without D; -inf for rows that see no key),
+    with which parts of an attention can be joined."""
+    return _decode(q, k_cache, v_cache, page_table, cache_seqlens, float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1]), True)
