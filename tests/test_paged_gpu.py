@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import varlenabsorbflashattn_b200 as vb
-from varlenabsorbflashattn_b200 import _lib
+from varlenabsorbflashattn_b200 import _lib, paged
 from paged_ref import assert_within, decode, paged_cache, positions_of, rotate, rotation_error
 
 pytestmark = pytest.mark.gpu
@@ -349,6 +349,7 @@ def test_decode_cut_otherwise(monkeypatch, sms):
     kc, vc, table = paged_cache(lens, 2, 64, 16, BF16, gen)
     q = _randn(gen, len(lens), 2, 6, 64, dtype=BF16)
     monkeypatch.setattr(_lib, "sm_count", lambda device: sms)
+    monkeypatch.setattr(paged, "_plans", {})
     _check_decode(q, kc, vc, table, lens, what=f"{sms} SMs")
 
 

@@ -18,9 +18,13 @@ int check_table(const float* cos, const float* sin, int R, int D, int rows) {
   return 0;
 }
 
-int check_cache(const void* k, const void* v, const int32_t* lens, const int32_t* table, int n_seq, int pages, int page_size, int max_pages) {
+int check_pointers(const void* k, const void* v, const int32_t* lens, const int32_t* table) {
   if (!k || !v) return fail(VAFA_ERR_INVALID, "null cache");
   if (!lens || !table) return fail(VAFA_ERR_INVALID, "null cache_seqlens/page_table");
+  return 0;
+}
+
+int check_cache(int n_seq, int pages, int page_size, int max_pages) {
   if (n_seq < 1 || pages < 1 || page_size < 1 || max_pages < 1)
     return fail(VAFA_ERR_INVALID, "bad sizes n_seq=%d num_pages=%d page_size=%d max_pages=%d", n_seq, pages, page_size, max_pages);
   if ((long long)max_pages * page_size > 0x7fffffffLL - 65536)
@@ -34,9 +38,8 @@ int check_decode(const vafa_paged_attn_args* a) {
   if (!dim_ok(a->head_dim)) return fail(VAFA_ERR_UNSUPPORTED, "head_dim %d not supported (16/32/64/128/256)", a->head_dim);
   if (a->q_len < 1 || a->num_heads < 1 || a->num_kv_heads < 1 || a->num_heads % a->num_kv_heads)
     return fail(VAFA_ERR_INVALID, "bad sizes q_len=%d H=%d H_kv=%d (H_kv must divide H)", a->q_len, a->num_heads, a->num_kv_heads);
-  if ((long long)a->q_len * a->num_heads > (1 << 20)) return fail(VAFA_ERR_UNSUPPORTED, "q_len %d x %d heads", a->q_len, a->num_heads);
-  if (const int rc = check_cache(a->k_cache, a->v_cache, a->cache_seqlens, a->page_table, a->n_seq, a->num_pages, a->page_size, a->max_pages)) return rc;
-  return 0;
+  if ((long long)a->q_len * a->num_heads > (1 << 20) || a->num_kv_heads > 0xffff) return fail(VAFA_ERR_UNSUPPORTED, "q_len %d x %d heads", a->q_len, a->num_heads);
+  return check_cache(a->n_seq, a->num_pages, a->page_size, a->max_pages);
 }
 
 paged::Plan plan_for(const vafa_paged_attn_args* a) {
@@ -98,6 +101,12 @@ int paged_decode_launch(const vafa_paged_attn_args* a, cudaStream_t s) {
   p.n_seq = a->n_seq; p.T = a->q_len; p.H = a->num_heads; p.H_kv = a->num_kv_heads;
   p.g = a->num_heads / a->num_kv_heads; p.R = p.T * p.g;
   p.row_tiles = plan.row_tiles; p.num_pages = a->num_pages; p.page_size = a->page_size;
+  // j / page_size by a product: page_mul = ceil(2^(32 + shift) / page_size) with 2^shift < page_size <= 2^(shift + 1) is off by less
+  // than page_size / 2^(32 + shift) <= 2^-31 of j, which stays below 1 / page_size of a step for j < 2^31
+  int shift = 0;
+  while ((1ll << (shift + 1)) <= a->page_size) ++shift;
+  p.page_shift = shift;
+  p.page_mul = (a->page_size & (a->page_size - 1)) == 0 ? 0 : (uint32_t)(((1ull << (32 + shift)) + a->page_size - 1) / a->page_size);
   p.capacity = a->max_pages * a->page_size;
   p.scale_log2 = a->scale * kLog2e;
   char* ws = (char*)a->workspace;
@@ -138,7 +147,8 @@ int vafa_paged_append(const vafa_paged_append_args* a, vafa_stream_t stream) {
   } else if (a->q) {
     return fail(VAFA_ERR_INVALID, "q without cos/sin");
   }
-  if ((rc = check_cache(a->k_cache, a->v_cache, a->cache_seqlens, a->page_table, a->n_seq, a->num_pages, a->page_size, a->max_pages))) return rc;
+  if ((rc = check_pointers(a->k_cache, a->v_cache, a->cache_seqlens, a->page_table))) return rc;
+  if ((rc = check_cache(a->n_seq, a->num_pages, a->page_size, a->max_pages))) return rc;
   if (!a->cu_seqlens && a->total != a->n_seq) return fail(VAFA_ERR_INVALID, "without cu_seqlens total %d must be n_seq %d", a->total, a->n_seq);
   if (a->total > 0 && (!a->k || !a->v || (a->q && !a->q_out))) return fail(VAFA_ERR_INVALID, "null k/v/q_out");
   return paged_append_launch(a, (cudaStream_t)stream);
@@ -151,6 +161,7 @@ size_t vafa_paged_decode_workspace_bytes(const vafa_paged_attn_args* a) {
 int vafa_paged_decode(const vafa_paged_attn_args* a, vafa_stream_t stream) {
   if (const int rc = check_decode(a)) return rc;
   if (!a->q || !a->o) return fail(VAFA_ERR_INVALID, "null q/o");
+  if (const int rc = check_pointers(a->k_cache, a->v_cache, a->cache_seqlens, a->page_table)) return rc;
   const int es = elem_size(a->dtype);
   auto of = [](int n, int64_t stride) { return n > 1 ? stride : 0; };  // (a dim of one element may have any stride)
   const int64_t strides = of(a->n_seq, a->q_seq_stride) | of(a->q_len, a->q_token_stride) | of(a->num_heads, a->q_head_stride) |

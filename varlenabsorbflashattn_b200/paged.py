@@ -85,7 +85,6 @@ def _check_angles(cos: torch.Tensor, sin: torch.Tensor, ref: torch.Tensor) -> in
     _need(cos.device == ref.device and sin.device == ref.device, lambda: "cos/sin must be on the device of q and k")
     _need(cos.is_contiguous() and sin.is_contiguous(), lambda: "cos/sin must be contiguous")
     _need(2 <= 2 * cos.shape[1] <= ref.shape[-1], lambda: f"rotary_dim {2 * cos.shape[1]} must be 2 to head_dim {ref.shape[-1]}")
-    _need(not (cos.requires_grad or sin.requires_grad), lambda: "cos/sin have no gradient here")
     return 2 * cos.shape[1]
 
 
@@ -131,6 +130,58 @@ def _check_pages(lens: torch.Tensor, table: torch.Tensor, num_pages: int, page_s
 
 
 # ------------------------------------------------------------------------------------------------
+# plans
+# ------------------------------------------------------------------------------------------------
+class _Plan:
+    """What the checks of a call make of its tensors' shapes, strides, types and devices: the argument struct but for the addresses.
+
+    A serving loop makes the same calls thousands of times and a check of each argument costs as much as the kernels of a
+    small step (35 us of a 40 us call), so calls of the same layout are checked once.  Nothing of the tensors' contents or addresses is in a plan."""
+    __slots__ = ("layout", "struct", "device", "index", "status", "call", "workspace", "out", "keep")
+
+    def __init__(self, struct, device, call, **more):
+        self.layout, self.struct = bytes(struct), type(struct)
+        self.device, self.index = device, device.index
+        self.keep = _lib.status_word(device)  # (held, so that its address stays)
+        self.status = self.keep.data_ptr()
+        self.call = getattr(_lib.load(), call)
+        self.workspace, self.out = more.get("workspace", 0), more.get("out")
+
+    def args(self):
+        a = self.struct.from_buffer_copy(self.layout)
+        a.status = self.status
+        return a
+
+    def run(self, a, what: str) -> None:
+        here = torch._C._cuda_getDevice() == self.index
+        if here:
+            rc = self.call(a, torch._C._cuda_getCurrentRawStream(self.index))
+        else:
+            with torch.cuda.device(self.device):
+                rc = self.call(a, torch._C._cuda_getCurrentRawStream(self.index))
+        if rc:
+            _lib.check(rc, what)
+        if _lib._check_after_each_op:
+            with _lib.on_device(self.device):
+                _lib.check_status(self.device)
+
+
+_plans: dict = {}
+_MOST_PLANS = 4096
+
+
+def _keep(key, plan: _Plan) -> _Plan:
+    if len(_plans) >= _MOST_PLANS:
+        _plans.clear()
+    _plans[key] = plan
+    return plan
+
+
+def _layout(t: Optional[torch.Tensor]):
+    return None if t is None else (t.shape, t.stride(), t.dtype, t.get_device())
+
+
+# ------------------------------------------------------------------------------------------------
 # rotation
 # ------------------------------------------------------------------------------------------------
 def rotary_table(positions: int, rotary_dim: int, *, base: float = 10000.0, device=None) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -147,22 +198,33 @@ def rotary_table(positions: int, rotary_dim: int, *, base: float = 10000.0, devi
     return angle.cos().float(), angle.sin().float()
 
 
-def _rotate(q, k, cos, sin, positions, cu, interleaved: bool, inverse: bool):
+def _rotary_plan(q, k, cos, positions, cu, interleaved: bool, inverse: bool) -> _Plan:
     ref = q if q is not None else k
     T, D = ref.shape[0], ref.shape[2]
     H, H_kv = (0 if x is None else x.shape[1] for x in (q, k))
-    qo = None if q is None else torch.empty((T, H, D), dtype=ref.dtype, device=ref.device)
-    ko = None if k is None else torch.empty((T, H_kv, D), dtype=ref.dtype, device=ref.device)
-    if T == 0:
-        return qo, ko
     qs, ks = ((0, 0) if x is None else x.stride()[:2] for x in (q, k))
-    a = _lib.RotaryArgs(
-        _lib.ptr(q), _lib.ptr(k), _lib.ptr(qo), _lib.ptr(ko), cos.data_ptr(), sin.data_ptr(), _lib.ptr(positions), _lib.ptr(cu),
-        *qs, *ks, 0 if cu is None else cu.numel() - 1, T, H, H_kv, D, 2 * cos.shape[1], cos.shape[0], _lib.DTYPE_CODE[ref.dtype],
-        interleaved, inverse, _lib.status_word(ref.device).data_ptr())
-    with _lib.on_device(ref.device):
-        _lib.check(_lib.load().vafa_rotary(a, _lib.raw_stream(ref.device)), "vafa_rotary")
-        _lib.maybe_check_status(ref.device)
+    a = _lib.RotaryArgs(*[None] * 8, *qs, *ks, 0 if cu is None else cu.numel() - 1, T, H, H_kv, D, 2 * cos.shape[1], cos.shape[0],
+                        _lib.DTYPE_CODE[ref.dtype], interleaved, inverse)
+    return _Plan(a, ref.device, "vafa_rotary", out=((T, H, D), (T, H_kv, D)))
+
+
+def _rotate(plan: _Plan, q, k, cos, sin, positions, cu):
+    shapes = plan.out
+    qo = None if q is None else q.new_empty(shapes[0])
+    ko = None if k is None else k.new_empty(shapes[1])
+    if shapes[0][0] == 0:
+        return qo, ko
+    a = plan.args()
+    if q is not None:
+        a.q, a.q_out = q.data_ptr(), qo.data_ptr()
+    if k is not None:
+        a.k, a.k_out = k.data_ptr(), ko.data_ptr()
+    a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
+    if cu is not None:
+        a.cu_seqlens = cu.data_ptr()
+    else:
+        a.positions = positions.data_ptr()
+    plan.run(a, "vafa_rotary")
     return qo, ko
 
 
@@ -170,24 +232,32 @@ class _PackedRotary(torch.autograd.Function):
     """y = R x per token and pair; the gradient is R^T dy, the rotation back, which has a gradient in turn."""
 
     @staticmethod
-    def forward(ctx, q, k, cos, sin, positions, cu, interleaved, inverse):
-        ctx.save_for_backward(cos, sin, positions, cu)
-        ctx.flags = interleaved, inverse
+    def forward(ctx, q, k, cos, sin, positions, cu, plan, interleaved, inverse):
+        ctx.save_for_backward(cos, sin, positions if cu is None else cu)
+        ctx.flags = cu is None, interleaved, inverse
         ctx.set_materialize_grads(False)
-        return _rotate(q, k, cos, sin, positions, cu, interleaved, inverse)
+        return _rotate(plan, q, k, cos, sin, positions, cu)
 
     @staticmethod
     def backward(ctx, dq, dk):
-        cos, sin, positions, cu = ctx.saved_tensors
-        interleaved, inverse = ctx.flags
-        dq = dq if dq is None or not ctx.needs_input_grad[0] or dq.stride(2) == 1 else dq.contiguous()
-        dk = dk if dk is None or not ctx.needs_input_grad[1] or dk.stride(2) == 1 else dk.contiguous()
-        dq = dq if ctx.needs_input_grad[0] else None
-        dk = dk if ctx.needs_input_grad[1] else None
+        cos, sin, where = ctx.saved_tensors
+        by_position, interleaved, inverse = ctx.flags
+        positions, cu = (where, None) if by_position else (None, where)
+        dq = _gradient(dq) if ctx.needs_input_grad[0] else None
+        dk = _gradient(dk) if ctx.needs_input_grad[1] else None
         if dq is None and dk is None:
-            return (None,) * 8
-        dq, dk = _PackedRotary.apply(dq, dk, cos, sin, positions, cu, interleaved, not inverse)
-        return dq, dk, None, None, None, None, None, None
+            return (None,) * 9
+        key = ("rotary", _layout(dq), _layout(dk), cos.shape, where.shape, by_position, interleaved, not inverse)
+        plan = _plans.get(key) or _keep(key, _rotary_plan(dq, dk, cos, positions, cu, interleaved, not inverse))
+        if torch.is_grad_enabled():
+            dq, dk = _PackedRotary.apply(dq, dk, cos, sin, positions, cu, plan, interleaved, not inverse)
+        else:
+            dq, dk = _rotate(plan, dq, dk, cos, sin, positions, cu)
+        return dq, dk, None, None, None, None, None, None, None
+
+
+def _gradient(d):
+    return d if d is None or d.stride(2) == 1 else d.contiguous()
 
 
 def packed_rotary(
@@ -215,27 +285,36 @@ def packed_rotary(
     A step with its gradients can be captured into a CUDA graph once validation is off; as with every operator, torch wants no
     eager autograd graph of the same leaves to be alive meanwhile (its AccumulateGrad nodes belong to the eager stream).
     """
-    q3, q4 = _rows(q, "q")
-    k3, k4 = (None, False) if k is None else _rows(k, "k")
-    _check_heads(q3, "q")
-    if k3 is not None:
-        _like(k3, q3, "k")
-        _need(k3.shape[0] == q3.shape[0] and k3.shape[2] == q3.shape[2], lambda: f"K shape mismatch: {tuple(k3.shape)} vs q {tuple(q3.shape)}")
-    _check_angles(cos, sin, q3)
-    T = q3.shape[0]
-    _lib.check_rows(T, cos.shape[0])
-    if (cu_seqlens is not None) + (seqinfo is not None) + (positions is not None) != 1:
-        raise ValueError("must provide one of cu_seqlens, seqinfo and positions")
-    if positions is None:
-        cu = _ints(cu_seqlens if seqinfo is None else _lengths_to_cu(seqinfo), q3.device, "cu_seqlens")
-        if cu.numel() < 2:
-            raise ValueError("cu_seqlens: must have at least 2 elements (n_seg+1 with n_seg>=1)")
-    else:
-        positions = _ints(positions, q3.device, "positions")
-        _need(positions.shape[0] == T, lambda: f"positions has {positions.shape[0]} entries for {T} tokens")
-        cu = None
+    if seqinfo is not None and cu_seqlens is None and positions is None:
+        cu_seqlens, seqinfo = _lengths_to_cu(seqinfo), None
+    key = ("packed_rotary", _layout(q), _layout(k), _layout(cos), _layout(sin), _layout(cu_seqlens), _layout(positions), seqinfo is None, interleaved)
+    plan = _plans.get(key)
+    q4 = k4 = False
+    if plan is None:
+        q, q4 = _rows(q, "q")
+        k, k4 = (None, False) if k is None else _rows(k, "k")
+        _check_heads(q, "q")
+        if k is not None:
+            _like(k, q, "k")
+            _need(k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2], lambda: f"K shape mismatch: {tuple(k.shape)} vs q {tuple(q.shape)}")
+        _check_angles(cos, sin, q)
+        _lib.check_rows(q.shape[0], cos.shape[0])
+        if (cu_seqlens is not None) + (seqinfo is not None) + (positions is not None) != 1:
+            raise ValueError("must provide one of cu_seqlens, seqinfo and positions")
+        if positions is None:
+            cu_seqlens = _ints(cu_seqlens, q.device, "cu_seqlens")
+            if cu_seqlens.numel() < 2:
+                raise ValueError("cu_seqlens: must have at least 2 elements (n_seg+1 with n_seg>=1)")
+        else:
+            positions = _ints(positions, q.device, "positions")
+            _need(positions.shape[0] == q.shape[0], lambda: f"positions has {positions.shape[0]} entries for {q.shape[0]} tokens")
+        plan = _rotary_plan(q, k, cos, positions, cu_seqlens, bool(interleaved), False)
+        # (a plan is for tensors as they came: none that was converted, copied or has a fourth dim)
+        if key[1:7] == (_layout(q), _layout(k), _layout(cos), _layout(sin), _layout(cu_seqlens), _layout(positions)):
+            _keep(key, plan)
+    T = q.shape[0]
     if _varlen._validate and T > 0:
-        host = _host(cu if positions is None else positions)
+        host = _host(cu_seqlens if positions is None else positions)
         if positions is None:
             _check_cu(host, T, "cu_seqlens")
             low, high = 0, int((host[1:] - host[:-1]).max()) - 1
@@ -243,10 +322,11 @@ def packed_rotary(
             low, high = int(host.min()), int(host.max())
         if low < 0 or high >= cos.shape[0]:
             raise ValueError(f"positions {low} to {high} leave the table of {cos.shape[0]}")
-    if torch.is_grad_enabled() and (q3.requires_grad or (k3 is not None and k3.requires_grad)):
-        qo, ko = _PackedRotary.apply(q3, k3, cos, sin, positions, cu, bool(interleaved), False)
+    if torch.is_grad_enabled() and (q.requires_grad or cos.requires_grad or sin.requires_grad or (k is not None and k.requires_grad)):
+        _need(not (cos.requires_grad or sin.requires_grad), lambda: "cos/sin have no gradient here")
+        qo, ko = _PackedRotary.apply(q, k, cos, sin, positions, cu_seqlens, plan, bool(interleaved), False)
     else:
-        qo, ko = _rotate(q3, k3, cos, sin, positions, cu, bool(interleaved), False)
+        qo, ko = _rotate(plan, q, k, cos, sin, positions, cu_seqlens)
     return (qo.unsqueeze(0) if q4 else qo), (ko.unsqueeze(0) if k4 else ko)
 
 
@@ -302,56 +382,73 @@ def paged_kv_append(
     Sequences may share pages that are only read (a common prefix); what is written must be theirs alone.
     Returns the rotated q (contiguous; zeros for padding), or None without q.  Has no gradient.
     """
-    k3, _ = _rows(k, "k")
-    v3, _ = _rows(v, "v")
-    _check_heads(k3, "k")
-    _like(v3, k3, "v")
-    _need(v3.shape == k3.shape, lambda: f"V shape mismatch: {tuple(v3.shape)} vs K {tuple(k3.shape)}")
-    T, H_kv, D = k3.shape
-    dev = k3.device
-    lens = _ints(cache_seqlens, dev, "cache_seqlens")
-    table = _ints(page_table, dev, "page_table", 2)
-    _check_cache(k_cache, v_cache, table, lens, k3)
-    num_pages, page_size = k_cache.shape[:2]
-    _need(k_cache.shape[2] == H_kv, lambda: f"caches have {k_cache.shape[2]} heads, k {H_kv}")
-    for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        _need(all(st > 0 or n == 1 for st, n in zip(c.stride(), c.shape)), lambda: f"{name}: an expanded tensor cannot be written to")
-    _need(k_cache.data_ptr() != v_cache.data_ptr(), lambda: "k_cache and v_cache are the same memory")
-    n_seq = lens.shape[0]
-    _lib.check_rows(T, n_seq)
-    cu = None
-    if cu_seqlens is not None or seqinfo is not None:
-        cu = _ints(cu_seqlens if cu_seqlens is not None else _lengths_to_cu(seqinfo), dev, "cu_seqlens")
-        _need(cu.shape[0] == n_seq + 1, lambda: f"cu_seqlens has {cu.shape[0] - 1} sequences, cache_seqlens {n_seq}")
-    else:
-        _need(T == n_seq, lambda: f"{T} new tokens for {n_seq} sequences need cu_seqlens or seqinfo")
-    if (cos is None) != (sin is None):
-        raise ValueError("cos and sin go together")
-    R = rows = 0
-    if cos is not None:
-        R, rows = _check_angles(cos, sin, k3), cos.shape[0]
-    q3, q4, qo = None, False, None
-    if q is not None:
-        if cos is None:
-            raise ValueError("q is rotated by cos and sin: without them it has nothing to do here")
-        q3, q4 = _rows(q, "q")
-        _like(q3, k3, "q")
-        _need(q3.shape[0] == T and q3.shape[2] == D, lambda: f"q shape mismatch: {tuple(q3.shape)} vs K {tuple(k3.shape)}")
-        _need(q3.shape[1] > 0, lambda: "q has no heads")
-    _no_gradient("paged_kv_append", k3, v3, q3, k_cache, v_cache)
-    if q3 is not None:
-        qo = torch.empty((T, q3.shape[1], D), dtype=q3.dtype, device=dev)
+    if seqinfo is not None and cu_seqlens is None:
+        cu_seqlens = _lengths_to_cu(seqinfo)
+    tensors = (k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens, q, cos, sin)
+    key = ("paged_kv_append", *map(_layout, tensors), interleaved)
+    plan = _plans.get(key)
+    q4 = False
+    if plan is None:
+        k, _ = _rows(k, "k")
+        v, _ = _rows(v, "v")
+        _check_heads(k, "k")
+        _like(v, k, "v")
+        _need(v.shape == k.shape, lambda: f"V shape mismatch: {tuple(v.shape)} vs K {tuple(k.shape)}")
+        T, H_kv, D = k.shape
+        dev = k.device
+        cache_seqlens = _ints(cache_seqlens, dev, "cache_seqlens")
+        page_table = _ints(page_table, dev, "page_table", 2)
+        _check_cache(k_cache, v_cache, page_table, cache_seqlens, k)
+        num_pages, page_size = k_cache.shape[:2]
+        _need(k_cache.shape[2] == H_kv, lambda: f"caches have {k_cache.shape[2]} heads, k {H_kv}")
+        for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+            _need(all(st > 0 or n == 1 for st, n in zip(c.stride(), c.shape)), lambda: f"{name}: an expanded tensor cannot be written to")
+        n_seq = cache_seqlens.shape[0]
+        _lib.check_rows(T, n_seq)
+        if cu_seqlens is not None:
+            cu_seqlens = _ints(cu_seqlens, dev, "cu_seqlens")
+            _need(cu_seqlens.shape[0] == n_seq + 1, lambda: f"cu_seqlens has {cu_seqlens.shape[0] - 1} sequences, cache_seqlens {n_seq}")
+        else:
+            _need(T == n_seq, lambda: f"{T} new tokens for {n_seq} sequences need cu_seqlens or seqinfo")
+        if (cos is None) != (sin is None):
+            raise ValueError("cos and sin go together")
+        R = rows = 0
+        if cos is not None:
+            R, rows = _check_angles(cos, sin, k), cos.shape[0]
+        if q is not None:
+            if cos is None:
+                raise ValueError("q is rotated by cos and sin: without them it has nothing to do here")
+            q, q4 = _rows(q, "q")
+            _like(q, k, "q")
+            _need(q.shape[0] == T and q.shape[2] == D, lambda: f"q shape mismatch: {tuple(q.shape)} vs K {tuple(k.shape)}")
+            _need(q.shape[1] > 0, lambda: "q has no heads")
+        a = _lib.PagedAppendArgs(
+            *[None] * 11, *((0, 0) if q is None else q.stride()[:2]), *k.stride()[:2], *v.stride()[:2], *k_cache.stride()[:3],
+            *v_cache.stride()[:3], page_table.stride(0), n_seq, T, 0 if q is None else q.shape[1], H_kv, D, R, rows, num_pages, page_size,
+            page_table.shape[1], _lib.DTYPE_CODE[k.dtype], bool(interleaved))
+        plan = _Plan(a, dev, "vafa_paged_append", out=(T, n_seq, None if q is None else (T, q.shape[1], D)))
+        if key[1:11] == tuple(map(_layout, (k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens, q, cos, sin))):
+            _keep(key, plan)
+    if torch.is_grad_enabled():
+        _no_gradient("paged_kv_append", k, v, q, k_cache, v_cache, cos, sin)
+    kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
+    _need(kc != vc, lambda: "k_cache and v_cache are the same memory")
+    T, n_seq, shape = plan.out
+    qo = None if q is None else q.new_empty(shape)
     if T > 0 and n_seq > 0:
         if _varlen._validate:
-            _check_append(_host(lens), _host(table), None if cu is None else _host(cu), T, num_pages, page_size, rows if R else None)
-        a = _lib.PagedAppendArgs(
-            _lib.ptr(q3), k3.data_ptr(), v3.data_ptr(), _lib.ptr(qo), k_cache.data_ptr(), v_cache.data_ptr(), _lib.ptr(cos), _lib.ptr(sin),
-            _lib.ptr(cu), lens.data_ptr(), table.data_ptr(), *((0, 0) if q3 is None else q3.stride()[:2]), *k3.stride()[:2], *v3.stride()[:2],
-            *k_cache.stride()[:3], *v_cache.stride()[:3], table.stride(0), n_seq, T, 0 if q3 is None else q3.shape[1], H_kv, D, R, rows,
-            num_pages, page_size, table.shape[1], _lib.DTYPE_CODE[k3.dtype], bool(interleaved), _lib.status_word(dev).data_ptr())
-        with _lib.on_device(dev):
-            _lib.check(_lib.load().vafa_paged_append(a, _lib.raw_stream(dev)), "vafa_paged_append")
-            _lib.maybe_check_status(dev)
+            _check_append(_host(cache_seqlens), _host(page_table), None if cu_seqlens is None else _host(cu_seqlens), T, k_cache.shape[0],
+                          k_cache.shape[1], None if cos is None else cos.shape[0])
+        a = plan.args()
+        a.k, a.v, a.k_cache, a.v_cache = k.data_ptr(), v.data_ptr(), kc, vc
+        a.cache_seqlens, a.page_table = cache_seqlens.data_ptr(), page_table.data_ptr()
+        if cu_seqlens is not None:
+            a.cu_seqlens = cu_seqlens.data_ptr()
+        if cos is not None:
+            a.cos, a.sin = cos.data_ptr(), sin.data_ptr()
+        if q is not None:
+            a.q, a.q_out = q.data_ptr(), qo.data_ptr()
+        plan.run(a, "vafa_paged_append")
     elif qo is not None:
         qo.zero_()
     return qo.unsqueeze(0) if q4 else qo
@@ -361,43 +458,58 @@ def paged_kv_append(
 # attention
 # ------------------------------------------------------------------------------------------------
 def _decode(q, k_cache, v_cache, page_table, cache_seqlens, scale, with_lse):
-    if q.dim() not in (3, 4):
-        raise ValueError(f"q: expected [n_seq,H,D] or [n_seq,T,H,D], got {q.dim()}-D")
-    _check_heads(q, "q")
-    dev = q.device
-    lens = _ints(cache_seqlens, dev, "cache_seqlens")
-    table = _ints(page_table, dev, "page_table", 2)
-    _check_cache(k_cache, v_cache, table, lens, q)
-    n_seq, H, D = q.shape[0], q.shape[-2], q.shape[-1]
-    T = q.shape[1] if q.dim() == 4 else 1
-    num_pages, page_size, H_kv = k_cache.shape[:3]
-    _need(n_seq == lens.shape[0], lambda: f"q has {n_seq} sequences, cache_seqlens {lens.shape[0]}")
-    _need(H % H_kv == 0, lambda: f"{H_kv} cache heads do not divide {H} query heads")
-    _no_gradient("paged_decode_attn", q, k_cache, v_cache)
-    es = q.element_size()
-    for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        if c.data_ptr() % 16 or any(n > 1 and st * es % 16 for st, n in zip(c.stride()[:3], c.shape)):
-            raise ValueError(f"{name}: base and strides must be multiples of 16 bytes")
-    if q.stride(-1) != 1 or q.data_ptr() % 16 or any(n > 1 and st * es % 16 for st, n in zip(q.stride()[:-1], q.shape)):
-        q = q.clone(memory_format=torch.contiguous_format)
-    o = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty(q.shape[:-1], dtype=torch.float32, device=dev) if with_lse else None
-    if o.numel() == 0:
+    tensors = (q, k_cache, v_cache, page_table, cache_seqlens)
+    key = ("paged_decode_attn", *map(_layout, tensors), scale)
+    plan = _plans.get(key)
+    if plan is None:
+        if q.dim() not in (3, 4):
+            raise ValueError(f"q: expected [n_seq,H,D] or [n_seq,T,H,D], got {q.dim()}-D")
+        _check_heads(q, "q")
+        dev = q.device
+        cache_seqlens = _ints(cache_seqlens, dev, "cache_seqlens")
+        page_table = _ints(page_table, dev, "page_table", 2)
+        _check_cache(k_cache, v_cache, page_table, cache_seqlens, q)
+        n_seq, H, D = q.shape[0], q.shape[-2], q.shape[-1]
+        T = q.shape[1] if q.dim() == 4 else 1
+        num_pages, page_size, H_kv = k_cache.shape[:3]
+        _need(n_seq == cache_seqlens.shape[0], lambda: f"q has {n_seq} sequences, cache_seqlens {cache_seqlens.shape[0]}")
+        _need(H % H_kv == 0, lambda: f"{H_kv} cache heads do not divide {H} query heads")
+        es = q.element_size()
+        for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+            if any(n > 1 and st * es % 16 for st, n in zip(c.stride()[:3], c.shape)):
+                raise ValueError(f"{name}: base and strides must be multiples of 16 bytes")
+        if q.stride(-1) != 1 or any(n > 1 and st * es % 16 for st, n in zip(q.stride()[:-1], q.shape)):
+            q = q.clone(memory_format=torch.contiguous_format)
+        st = q.stride()
+        a = _lib.PagedAttnArgs(
+            *[None] * 7, st[0], st[1] if q.dim() == 4 else 0, st[-2], *k_cache.stride()[:3], *v_cache.stride()[:3], page_table.stride(0),
+            n_seq, T, H, H_kv, D, num_pages, page_size, page_table.shape[1], _lib.DTYPE_CODE[q.dtype],
+            1.0 / math.sqrt(D) if scale is None else scale, _lib.sm_count(dev))
+        plan = _Plan(a, dev, "vafa_paged_decode", workspace=_lib.load().vafa_paged_decode_workspace_bytes(a) if q.numel() else 0,
+                     out=(tuple(q.shape[:-1]), q.numel()))
+        if key[1:6] == tuple(map(_layout, (q, k_cache, v_cache, page_table, cache_seqlens))):
+            _keep(key, plan)
+    if torch.is_grad_enabled():
+        _no_gradient("paged_decode_attn", q, k_cache, v_cache)
+    kc, vc, qp = k_cache.data_ptr(), v_cache.data_ptr(), q.data_ptr()
+    if (kc | vc) & 15:
+        raise ValueError("k_cache, v_cache: base and strides must be multiples of 16 bytes")
+    if qp & 15:
+        return _decode(q.clone(), k_cache, v_cache, page_table, cache_seqlens, scale, with_lse)
+    o = q.new_empty(q.shape)
+    lse = torch.empty(plan.out[0], dtype=torch.float32, device=plan.device) if with_lse else None
+    if plan.out[1] == 0:
         return o, lse
     if _varlen._validate:
-        _check_pages(_host(lens), _host(table), num_pages, page_size)
-    lib = _lib.load()
-    st = q.stride()
-    with _lib.on_device(dev):
-        a = _lib.PagedAttnArgs(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), _lib.ptr(lse), lens.data_ptr(), table.data_ptr(),
-            st[0], st[1] if q.dim() == 4 else 0, st[-2], *k_cache.stride()[:3], *v_cache.stride()[:3], table.stride(0),
-            n_seq, T, H, H_kv, D, num_pages, page_size, table.shape[1], _lib.DTYPE_CODE[q.dtype], scale, _lib.sm_count(dev),
-            None, 0, _lib.status_word(dev).data_ptr())
-        ws = _lib.workspace(lib.vafa_paged_decode_workspace_bytes(a), dev)
-        a.workspace, a.workspace_bytes = _lib.ptr(ws), 0 if ws is None else ws.numel()
-        _lib.check(lib.vafa_paged_decode(a, _lib.raw_stream(dev)), "vafa_paged_decode")
-        _lib.maybe_check_status(dev)
+        _check_pages(_host(cache_seqlens), _host(page_table), k_cache.shape[0], k_cache.shape[1])
+    a = plan.args()
+    a.q, a.k_cache, a.v_cache, a.o = qp, kc, vc, o.data_ptr()
+    a.cache_seqlens, a.page_table = cache_seqlens.data_ptr(), page_table.data_ptr()
+    if lse is not None:
+        a.lse = lse.data_ptr()
+    ws = torch.empty(plan.workspace, dtype=torch.uint8, device=plan.device)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), plan.workspace
+    plan.run(a, "vafa_paged_decode")
     return o, lse
 
 
@@ -422,10 +534,10 @@ def paged_decode_attn(
     joined in a fixed order: the same call gives the same bits, another batch around a sequence may round
     differently.  Meant for few new tokens; a prompt's own attention is `packed_varlen_attn`.  Has no gradient.
     """
-    return _decode(q, k_cache, v_cache, page_table, cache_seqlens, float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1]), False)[0]
+    return _decode(q, k_cache, v_cache, page_table, cache_seqlens, None if scale is None else float(scale), False)[0]
 
 
 def paged_decode_attn_with_lse(q, k_cache, v_cache, *, page_table, cache_seqlens, scale=None):
     """As paged_decode_attn, and also returns the natural-log LSE (fp32, q's shape without D; -inf for rows that see no key),
     with which parts of an attention can be joined."""
-    return _decode(q, k_cache, v_cache, page_table, cache_seqlens, float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1]), True)
+    return _decode(q, k_cache, v_cache, page_table, cache_seqlens, None if scale is None else float(scale), True)
