@@ -597,3 +597,62 @@ def test_the_kernels_of_this_library_ran():
     after = {n: v[2] for n, v in _lib.profile_read().items()}
     for name in ("rotary_kernel", "rotary_kernel<append>", "paged_decode_kernel", "paged_combine_kernel"):
         assert after.get(name, 0) == before.get(name, 0) + 1, name
+
+
+# ---- long batches: rows through shared memory ---------------------------------------------------------------
+@pytest.mark.parametrize("dtype,H,H_kv,D,R,interleaved,view", [
+    (BF16, 32, 8, 128, 128, False, False), (F16, 32, 8, 128, 64, True, True), (F32, 8, 2, 64, 58, False, False), (BF16, 8, 8, 64, 64, False, True),
+    (F16, 7, 1, 256, 100, True, False), (F32, 4, 4, 128, 128, True, True), (BF16, 20, 5, 32, 30, False, False)])
+def test_rotary_and_append_of_long_batches(dtype, H, H_kv, D, R, interleaved, view):
+    """Batches over the size from which token rows go through shared memory, their last tile part full."""
+    gen = _gen(H + D)
+    T = (11 << 20) // ((H + H_kv) * D * dtype.itemsize) + 3
+    lens = [1, 0, 700, 5, 33]
+    lens.append(T - sum(lens))
+    qkv = _randn(gen, T, H + 2 * H_kv, D, dtype=dtype)
+    q, k, v = qkv[:, :H], qkv[:, H:H + H_kv], qkv[:, H + H_kv:]
+    if not view:
+        q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    cos, sin = vb.rotary_table(max(lens), R, device="cuda")
+    pos = positions_of(lens).cuda()
+    before = sum(x[2] for n, x in _lib.profile_read().items() if n == "rotary_kernel<rows>")
+    out = vb.packed_rotary(q, k, cos, sin, cu_seqlens=_cu(lens), interleaved=interleaved)
+    for name, x, y in zip("qk", (q, k), out):
+        ref, mag = rotate(x, cos, sin, pos, interleaved)
+        assert_within(y, ref, rotation_error(ref, mag, dtype), name)
+    assert torch.equal(vb.packed_rotary(q, None, cos, sin, positions=pos, interleaved=interleaved)[0], out[0])
+    for page, layout in ((16, "nhd"), (7, "hnd")):
+        kc, vc, table = paged_cache(lens, H_kv, D, page, dtype, gen, layout=layout, fill=7.0)
+        want = _append_ref(out[1], v, kc, vc, table, pos, torch.repeat_interleave(torch.arange(6), torch.tensor(lens)).cuda(), page)
+        got = vb.paged_kv_append(k, v, kc, vc, page_table=table, cache_seqlens=_ints(lens), cu_seqlens=_cu(lens), q=q, cos=cos, sin=sin,
+                                 interleaved=interleaved)
+        assert torch.equal(got, out[0]) and torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+        vb.paged_kv_append(out[1], v, kc, vc, page_table=table, cache_seqlens=_ints(lens), cu_seqlens=_cu(lens))
+        assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+    assert sum(x[2] for n, x in _lib.profile_read().items() if n == "rotary_kernel<rows>") >= before + 3
+
+
+def test_long_batches_with_rows_behind_padding_and_bad_places(unchecked):
+    gen, H, D = _gen(31), 8, 128
+    T = 6000
+    q, k, v = (_randn(gen, T, H, D, dtype=BF16) for _ in range(3))
+    cos, sin = vb.rotary_table(3000, D, device="cuda")
+    lens = [1500, 100, 2500]  # 1900 rows behind
+    _status()
+    a, b = vb.packed_rotary(q, k, cos, sin, cu_seqlens=_cu(lens))
+    assert (a[4100:] == 0).all() and (b[4100:] == 0).all() and _status() == [0, 0]
+    pos = positions_of(lens).cuda()
+    short = vb.packed_rotary(q[:4100], k[:4100], cos, sin, positions=pos)
+    assert torch.equal(a[:4100], short[0]) and torch.equal(b[:4100], short[1])
+    kc, vc, table = paged_cache([1500, 100, 2500], H, D, 16, BF16, gen, fill=0.0)
+    before, bad = (kc.clone(), vc.clone()), table.clone()
+    bad[0, 40] = kc.shape[0]
+    got = vb.paged_kv_append(k, v, kc, vc, page_table=bad, cache_seqlens=_ints([1500, 0, 2500]), cu_seqlens=_cu(lens), q=q, cos=cos, sin=sin)
+    assert _status() == [4, 911]
+    assert got[640:656].isnan().all() and (got[1500:1600] == 0).all() and (got[4100:] == 0).all()
+    keep = torch.ones(4100, dtype=torch.bool, device="cuda")
+    keep[640:656] = keep[1500:1600] = False
+    assert torch.equal(got[:4100][keep], a[:4100][keep])
+    seq = torch.repeat_interleave(torch.arange(3), torch.tensor(lens)).cuda()
+    want = _append_ref(b[:4100][keep], v[:4100][keep], *before, table, pos[keep], seq[keep], 16)
+    assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])

@@ -8,7 +8,6 @@ namespace vafa {
 constexpr int kBadCacheIndex = 4;
 constexpr int kSiteRotary = 910, kSiteAppend = 911, kSiteDecode = 912;
 
-// The rotation kernel's work: `n_rot` groups of heads to rotate (queries, keys) and one to copy (values).
 int rotary_launch(const vafa_rotary_args* a, cudaStream_t s);
 int paged_append_launch(const vafa_paged_append_args* a, cudaStream_t s);
 

@@ -27,6 +27,7 @@ enum KernelId {
   kKBwdDqFin,
   kKAbsorbBwdDxu,
   kKRotary,
+  kKRotaryRows,
   kKPagedAppend,
   kKPagedDecode,
   kKPagedCombine,
