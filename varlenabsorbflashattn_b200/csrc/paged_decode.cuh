@@ -11,60 +11,32 @@
 //    result does not depend on timing.  Each CTA finds its piece from the lengths itself: nothing is read on the host.
 //  - K and V blocks are copied to shared memory by cp.async, S blocks deep, 16 bytes at a time, because a page may
 //    be of any size and end inside a block; page ids are read two blocks before they are needed.
-//  - 16-bit types use m16n8k16 products with the keys (then the head dim) as their 16 rows and the query rows as their 8 columns:
-//    a single token of up to 8 grouped heads fills the tile, where 128-row tcgen05 tiles would be 1/128 to 1/16 full.
-//    The products are far from the tensor pipe's limit (see the table in the notes), so the legacy instruction costs nothing.
-//  - each of the KW warps of a row group owns 16 (fp32: 8 or 16) keys of a block with its own maximum and sum, so the loop has no
-//    exchange between warps; they are joined once, at the unit's end.
-// P is split into two 16-bit pieces (hi + lo) for the second product: one piece would put an error of the size of the
-// output's own rounding on top of it, the second costs one more product per V fragment and no time.
+//  - each warp has its own keys of a block with its own maximum and sum (paged_decode_tiles.cuh), so that the loop has no exchange
+//    between warps; they are joined once, at the unit's end.
 #pragma once
 #include <atomic>
-#include <type_traits>
 
-#include "paged_kernels.cuh"
+#include "paged_decode_tiles.cuh"
 #include "profile.cuh"
 
-#ifndef PD_CTAS
-#define PD_CTAS 3
-#endif
-#ifndef PD_UNIT
-#define PD_UNIT 2
-#endif
-#ifndef PD_KW
-#define PD_KW 4
-#endif
-#ifndef PD_MAXS
-#define PD_MAXS 6
-#endif
 namespace vafa {
 namespace paged {
 
-struct DecodeParams {
-  const void* q; const void* k; const void* v;
-  void* o; float* lse;
-  const int32_t* lens; const int32_t* table;
-  int64_t q_seq, q_token, q_head;
-  int64_t k_page, k_slot, k_head, v_page, v_slot, v_head;
-  int64_t table_stride;
-  int n_seq, T, H, H_kv, g, R;            // g = H / H_kv, R = T * g rows of a unit
-  int row_tiles, num_pages, page_size;
-  uint32_t page_mul; int page_shift;      // j / page_size = (j * page_mul) >> 32 >> page_shift for j below 2^31 (page_mul 0: a shift alone)
-  int capacity;                           // keys that a row of the page table holds
-  float scale_log2;
-  float* part_o; float2* part_ml; int4* meta;
-  int32_t* status;
-};
-
-template <typename T_, int D_, int NT_, int RG_, int KW_>
+// How a shape is cut: RG groups of KW warps, a group's warps share out the keys of a block and have ROWS_G rows each; at most MOST CTAs an SM.
+enum Kind { kNarrow, kWide, kSingle };  // (kSingle: fp32)
+template <typename T_, int D_, Kind KIND_, int RG_, int KW_, int MOST_>
 struct Config {
   using T = T_;
-  static constexpr int D = D_, NT = NT_, RG = RG_, KW = KW_;
-  static constexpr bool kFp32 = sizeof(T) == 4;
-  static constexpr int KPW = kFp32 && D >= 128 ? 8 : 16;   // keys of a warp
+  static constexpr int D = D_, RG = RG_, KW = KW_;
+  static constexpr Kind KIND = KIND_;
+  static constexpr bool kFp32 = KIND == kSingle;
+  static_assert(kFp32 == (sizeof(T) == 4), "fp32 has a tile of its own");
+  static constexpr int NT = KIND == kWide ? 2 : 1;           // groups of 8 rows of a warp
+  static constexpr int KPW = kFp32 ? (D >= 128 ? 8 : 16) : KIND == kWide ? 64 / KW : D <= 64 ? 32 : 16;  // keys of a warp
   static constexpr int BK = KW * KPW;
   static constexpr int ROWS_G = 8 * NT, ROWS = ROWS_G * RG;
   static constexpr int THREADS = 32 * KW * RG;
+  static_assert(BK <= THREADS, "a thread looks up a key's place");
   static constexpr int VEC = 16 / (int)sizeof(T), CH = D / VEC;
   // A row's 16-byte chunks are stored at chunk ^ key(row): the 8 rows that an ldmatrix tile (fp32: the 2 rows that 8 lanes)
   // read at the same chunk then lie in different banks without padding.
@@ -74,33 +46,34 @@ struct Config {
     else return (row / (CH < 8 ? 8 / CH : 1)) & ((CH < 8 ? CH : 8) - 1);
   }
   static constexpr int kStageBytes = (2 * BK + ROWS) * PITCH;
-  static constexpr bool kQReg = !kFp32 && (RG == 1 || (RG == 2 && D <= 64));  // Q fragments stay in registers
+  static constexpr bool kQReg = KIND == kNarrow || (KIND == kWide && D <= 128);  // Q fragments stay in registers
   static constexpr int kQBytes = kQReg ? 0 : ROWS * PITCH;
-  static constexpr int MP = D + 4;                         // pitch of the join buffer, floats: 8 rows of each warp of a row group
+  static constexpr int MP = KIND == kWide ? D + 8 : D + 4;                         // pitch of the join buffer, floats: 8 rows of each warp of a row group
   static constexpr int kJoinBytes = KW * 8 * MP * 4;
   static_assert(kJoinBytes <= kStageBytes, "the join buffer takes the place of a stage that has been read");
   static constexpr int kMlBytes = RG * KW * ROWS_G * 8;
   static constexpr int kPBytes = kFp32 ? RG * KW * (KPW + 2) * 8 * 4 : 0;
   static constexpr int kBudget = 227 * 1024;
-  static constexpr int kMaxStages = PD_MAXS;
+  static constexpr int kMaxStages = 6;
   static constexpr int bytes_of(int s) { return s * kStageBytes + kQBytes + kMlBytes + kPBytes + (s + 2) * (16 + BK * 16) + 256; }
   static constexpr int fit(int ctas) {
     int s = kMaxStages;
     while (s > 1 && (bytes_of(s) + 1024) * ctas > kBudget + 1024) --s;
     return s;
   }
-  // CTAs of an SM, as far as registers and shared memory go
-  static constexpr int CTAS = RG == 1 && NT == 1 && fit(PD_CTAS) >= 2 ? PD_CTAS : RG <= 2 && !(D == 256) && fit(2) >= 2 ? 2 : 1;
+  static constexpr int CTAS = MOST_ >= 4 && fit(4) >= 2 ? 4 : MOST_ >= 3 && fit(3) >= 2 ? 3 : MOST_ >= 2 && fit(2) >= 2 ? 2 : 1;
+  static constexpr int kRegisters = 65536 / (THREADS * CTAS);
   static constexpr int S = fit(CTAS);
   static constexpr int kInfo = S + 2;                      // slots of the ring of block descriptions
   static_assert(S >= 2, "no room for two stages");
   static constexpr int kSmem = bytes_of(S);
+  using Tile = std::conditional_t<kFp32, Fp32Tile<Config>, std::conditional_t<KIND == kWide, WideTile<Config>, NarrowTile<Config>>>;
 };
 
 // A piece of the line of blocks: what a CTA needs to know to find its first block.  A unit costs more than its blocks (its
 // queries, the join of the warps, the rows' way out), so the line that is cut has `kUnitCost` slots more in front of each
 // unit's blocks; a piece that begins or ends among those begins or ends with the unit's first block.
-constexpr int kUnitCost = PD_UNIT;
+constexpr int kUnitCost = 2;
 struct Piece {
   long long first, last;      // blocks [first, last), the slots not counted
   long long share;            // slots and blocks of a piece
@@ -177,73 +150,6 @@ __device__ void find_piece(const DecodeParams& p, Piece* out, long long* scan, i
   __syncthreads();
 }
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-// 16 bytes to shared memory; zeros where there is nothing to read.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
-  const int n = real ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n));  // (no memory clobber: the places of later rows may be read meanwhile)
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
-}
-__device__ __forceinline__ void ldsm2(uint32_t& r0, uint32_t& r1, uint32_t a) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(a) : "memory");
-}
-__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-  return y;
-}
-template <typename T>
-__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if constexpr (sizeof(T) == 2) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value)
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-    else
-      asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                   : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-}
-// Whether one of two 16-bit values is infinite or NaN: its exponent is all ones.
-template <typename T>
-__device__ __forceinline__ bool not_finite2(uint32_t x) {
-  constexpr uint32_t e = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
-  return (x & e) == e || (x & (e << 16)) == (e << 16);
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-// The weight of a partial sum with maximum m beside a maximum `all`: nothing where there is nothing.
-__device__ __forceinline__ float weight(float m, float all) { return m == -INFINITY ? 0.f : exp2_approx(m - all); }
-
-template <typename T>
-__device__ __forceinline__ void store4(T* dst, float4 x) {
-  if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = x;
-  else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2_out<T>(x.x, x.y), pack2_out<T>(x.z, x.w));
-}
-// Four values of a finished row.  A row that sees no key is zero; one whose every score is -inf is 0 / 0, as in the formula.
-template <typename T>
-__device__ __forceinline__ void write_row(const DecodeParams& p, int seq, int h, int r, int len, int D, int d, float4 sum, float m, float l) {
-  const int t = r / p.g;
-  const int64_t row = ((int64_t)seq * p.T + t) * p.H + h * p.g + r - t * p.g;
-  const bool sees = len - p.T + t + 1 > 0;
-  const float inv = 1.f / l;
-  store4(reinterpret_cast<T*>(p.o) + row * D + d,
-         sees ? make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv) : make_float4(0.f, 0.f, 0.f, 0.f));
-  if (p.lse != nullptr && d == 0) p.lse[row] = sees ? (m + log2f(l)) * 0.69314718055994531f : -INFINITY;
-}
-
 __device__ __forceinline__ int page_of(const DecodeParams& p, int j) {
   return p.page_mul ? (int)(__umulhi((uint32_t)j, p.page_mul) >> p.page_shift) : j >> p.page_shift;
 }
@@ -255,8 +161,7 @@ struct Block {  // a block of the line, as its ring slot describes it
 template <typename C>
 __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const DecodeParams p, int min_share) {
   using T = typename C::T;
-  constexpr int D = C::D, NT = C::NT, RG = C::RG, BK = C::BK, KW = C::KW, S = C::S, KPW = C::KPW;
-  constexpr bool kFp32 = C::kFp32;
+  constexpr int D = C::D, NT = C::NT, RG = C::RG, BK = C::BK, KW = C::KW, S = C::S;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Piece piece;
   __shared__ long long scan[C::THREADS / 32];
@@ -380,20 +285,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
     copy_commit();
   }
 
-  // ---- state of the unit under way ----
-  float o[kFp32 ? 8 : D / 16 * NT][kFp32 ? (D + 31) / 32 : 4];
-  float m[2 * NT], l[2 * NT];          // of the columns (rows of the unit) 8 nt + 2 (lane % 4) + {0, 1}
-  int limit[2 * NT];                   // keys that the row sees
-  uint32_t qf[C::kQReg ? D / 16 : 1][NT][2];
-  constexpr int kMost = C::THREADS * C::CTAS >= 512 ? 4 : 8;
-  constexpr int kAhead = D / 16 < kMost ? D / 16 : kMost;      // fragments of K or V in flight, as registers allow
-  const int key0 = kw * KPW;                                   // the warp's keys of a block
-  const int k_row = (key0 + (lane & 15)) * C::PITCH, k_key = C::key(lane & 15);
-  const int v_row = (key0 + (lane & 7) + ((lane >> 4) & 1) * 8) * C::PITCH, v_key = C::key((lane & 7) + ((lane >> 4) & 1) * 8);
-  auto q_addr = [&](uint32_t base, int nt, int d) {
-    return base + (rg * C::ROWS_G + nt * 8 + (lane & 7)) * C::PITCH + (((2 * d + ((lane >> 3) & 1)) ^ C::key(lane & 7)) << 4);
-  };
-  float* const p_warp = p_all + warp * (KPW + 2) * 8;
+  typename C::Tile tile(Place{lane, kw, rg});
   int unit_kb0 = 0;                    // first block of the unit that this CTA has
 
   for (int i = 0; i < n_iter; ++i) {
@@ -408,291 +300,28 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
     }
     const Block b = info[i % C::kInfo];
     unsigned char* const st = stages + (i % S) * C::kStageBytes;
-    const uint32_t ks = smem_addr(st), vs = ks + BK * C::PITCH, qs = vs + BK * C::PITCH;
     const int nb = blocks_of<BK>(b.len);
     const int h = b.hr & 0xffff, row0 = (b.hr >> 16) * C::ROWS;
 
     if (i == 0 || b.kb == 0) {
       unit_kb0 = b.kb;
-#pragma unroll
-      for (int x = 0; x < 2 * NT; ++x) {
-        m[x] = -INFINITY;
-        l[x] = 0.f;
-        const int r = row0 + rg * C::ROWS_G + (x >> 1) * 8 + 2 * (lane & 3) + (x & 1);
-        limit[x] = min(b.len, b.len - p.T + min(r, p.R - 1) / p.g + 1);
-      }
-#pragma unroll
-      for (int x = 0; x < (int)(sizeof(o) / sizeof(o[0])); ++x)
-#pragma unroll
-        for (int y = 0; y < (int)(sizeof(o[0]) / 4); ++y) o[x][y] = 0.f;
-      if constexpr (C::kQReg) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d)
-            ldsm2(qf[d][nt][0], qf[d][nt][1], q_addr(qs, nt, d));
-      } else {
-        for (int e = tid; e < C::ROWS * C::CH; e += C::THREADS) {
-          *reinterpret_cast<uint4*>(q_now + e * 16) = *reinterpret_cast<const uint4*>(st + 2 * BK * C::PITCH + e * 16);
-        }
+      const unsigned char* q = st + 2 * BK * C::PITCH;
+      if constexpr (!C::kQReg) {  // the stage goes, the queries stay
+        for (int e = tid; e < C::ROWS * C::CH; e += C::THREADS)
+          *reinterpret_cast<uint4*>(q_now + e * 16) = *reinterpret_cast<const uint4*>(q + e * 16);
         __syncthreads();
+        q = q_now;
       }
+      tile.begin(p, q, b.len, row0, p_all + warp * (C::KPW + 2) * 8);
     }
-
-    // ---- scores: s[nt][2 e + x] = key 8 e + lane / 4 of the warp's, column 8 nt + 2 (lane % 4) + x ----
-    float s[NT][4];
-    if constexpr (kFp32) {
-      constexpr int KL = KPW / 8;
-      float acc[KL][8];
-#pragma unroll
-      for (int e = 0; e < KL; ++e)
-#pragma unroll
-        for (int r = 0; r < 8; ++r) acc[e][r] = 0.f;
-      const unsigned char* const kr = st + (key0 + (lane >> 2)) * C::PITCH;  // (keys 8 apart have the same key())
-      const unsigned char* const qr = q_now + rg * 8 * C::PITCH;
-      const int ck = C::key(lane >> 2);
-#pragma unroll 4
-      for (int d = 0; d < D / 16; ++d) {
-        float4 kv[KL];
-#pragma unroll
-        for (int e = 0; e < KL; ++e) kv[e] = *reinterpret_cast<const float4*>(kr + e * 8 * C::PITCH + ((4 * d + (lane & 3)) ^ ck) * 16);
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const float4 qv = *reinterpret_cast<const float4*>(qr + r * C::PITCH + ((4 * d + (lane & 3)) ^ C::key(r)) * 16);
-#pragma unroll
-          for (int e = 0; e < KL; ++e)
-            acc[e][r] = fmaf(qv.x, kv[e].x, fmaf(qv.y, kv[e].y, fmaf(qv.z, kv[e].z, fmaf(qv.w, kv[e].w, acc[e][r]))));
-        }
-      }
-      // the four lanes of a key sum their quarters; lane % 4 keeps rows 2 (lane % 4) and the next
-#pragma unroll
-      for (int e = 0; e < KL; ++e) {
-        float h4[4];
-        const bool hi2 = (lane & 2) != 0, hi1 = (lane & 1) != 0;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float give = hi2 ? acc[e][r] : acc[e][r + 4], keep = hi2 ? acc[e][r + 4] : acc[e][r];
-          h4[r] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
-        }
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float give = hi1 ? h4[r] : h4[r + 2], keep = hi1 ? h4[r + 2] : h4[r];
-          s[0][2 * e + r] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
-        }
-      }
-      if constexpr (KL == 1) s[0][2] = s[0][3] = -INFINITY;
-    } else {
-      // K fragments are all on their way before the first product, V's first ones before the softmax; even and odd steps of the
-      // head dim are summed apart, which halves the chain of dependent products
-      float odd[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[nt][x] = odd[nt][x] = 0.f;
-#pragma unroll
-      for (int d0 = 0; d0 < D / 16; d0 += kAhead) {
-        uint32_t a[kAhead][4];
-#pragma unroll
-        for (int d = 0; d < kAhead; ++d)
-          ldsm4(a[d], ks + k_row + (((2 * (d0 + d) + (lane >> 4)) ^ k_key) << 4));
-#pragma unroll
-        for (int d = 0; d < kAhead; ++d)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            uint32_t b0, b1;
-            if constexpr (C::kQReg) {
-              b0 = qf[d0 + d][nt][0];
-              b1 = qf[d0 + d][nt][1];
-            } else {
-              ldsm2(b0, b1, q_addr(smem_addr(q_now), nt, d0 + d));
-            }
-            mma<T>((d & 1) ? odd[nt] : s[nt], a[d], b0, b1);
-          }
-      }
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) s[nt][x] += odd[nt][x];
-    }
-    uint32_t va[kFp32 ? 1 : kAhead][4];
-    if constexpr (!kFp32) {
-#pragma unroll
-      for (int d = 0; d < kAhead; ++d) ldsm4t(va[d], vs + v_row + (((2 * d + ((lane >> 3) & 1)) ^ v_key) << 4));
-    }
-
-    // ---- softmax ----
-    const int j0 = b.kb * BK + key0 + (lane >> 2);                // the lane's first key
-    const int every = b.len - p.T + 1;                            // keys below this one are seen by every row
-    const bool masked = (b.kb + 1) * BK > every;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int x = 0; x < 4; ++x) {
-        s[nt][x] *= p.scale_log2;
-        if (masked && (j0 + (x >> 1) * 8 >= limit[2 * nt + (x & 1)])) s[nt][x] = -INFINITY;
-        if (kFp32 && KPW == 8 && x >= 2) s[nt][x] = -INFINITY;
-      }
-    float alpha[2 * NT];
-    bool moved = false;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float top = fmaxf(s[nt][x], s[nt][x + 2]);
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        const int c = 2 * nt + x;
-        const float now = fmaxf(m[c], top);
-        moved |= now != m[c];
-        alpha[c] = weight(m[c], now);
-        const float ref = now == -INFINITY ? 0.f : now;
-        s[nt][x] = exp2_approx(s[nt][x] - ref);
-        s[nt][x + 2] = exp2_approx(s[nt][x + 2] - ref);
-        l[c] = l[c] * alpha[c] + (s[nt][x] + s[nt][x + 2]);
-        m[c] = now;
-      }
-
-    // ---- O = alpha O + P V ----
-    // Keys that some rows see and others do not are summed apart where V is not finite: 0 times a NaN would reach the others.
-    const int apart0 = p.T > 1 && masked ? max(0, every - (b.kb * BK + key0)) : KPW;
-    const int apart1 = min(KPW, b.len - (b.kb * BK + key0));
-    if constexpr (kFp32) {
-      constexpr int DV = (D + 31) / 32;
-      float* const pr = p_warp;
-      __syncwarp();
-#pragma unroll
-      for (int e = 0; e < KPW / 8; ++e)
-        *reinterpret_cast<float2*>(pr + (8 * e + (lane >> 2)) * 8 + 2 * (lane & 3)) = make_float2(s[0][2 * e], s[0][2 * e + 1]);
-      if (lane < 4) *reinterpret_cast<float2*>(pr + KPW * 8 + 2 * lane) = make_float2(alpha[0], alpha[1]);
-      if (lane < 4) *reinterpret_cast<int2*>(pr + (KPW + 1) * 8 + 2 * lane) = make_int2(limit[0], limit[1]);
-      __syncwarp();
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const float f = pr[KPW * 8 + r];
-#pragma unroll
-          for (int y = 0; y < DV; ++y) o[r][y] *= f;
-        }
-      }
-      constexpr int W = D >= 128 ? 4 : D / 32 > 0 ? D / 32 : 1;  // floats of one read
-      const unsigned char* const vr = st + (BK + key0) * C::PITCH;
-      const bool has = D >= 32 || lane < D;
-#pragma unroll 4
-      for (int k = 0; k < KPW; ++k) {
-        const float4 pa = *reinterpret_cast<const float4*>(pr + k * 8), pb = *reinterpret_cast<const float4*>(pr + k * 8 + 4);
-        const float pk[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
-        float v[DV];
-        const unsigned char* const row = vr + k * C::PITCH;
-        const int ck = C::key(k);
-#pragma unroll
-        for (int y = 0; y < DV; y += W) {
-          const int ch = y * 8 + lane * W / 4;
-          const float* const x = reinterpret_cast<const float*>(row + (ch ^ ck) * 16) + lane * W % 4;
-          if constexpr (W == 4) {
-            const float4 f = *reinterpret_cast<const float4*>(x);
-            v[y] = f.x; v[y + 1] = f.y; v[y + 2] = f.z; v[y + 3] = f.w;
-          } else if constexpr (W == 2) {
-            const float2 f = *reinterpret_cast<const float2*>(x);
-            v[y] = f.x; v[y + 1] = f.y;
-          } else {
-            v[y] = has ? *x : 0.f;
-          }
-        }
-        if (k < apart0) {
-#pragma unroll
-          for (int r = 0; r < 8; ++r)
-#pragma unroll
-            for (int y = 0; y < DV; ++y) o[r][y] = fmaf(pk[r], v[y], o[r][y]);
-        } else {
-          const int j = b.kb * BK + key0 + k;
-#pragma unroll
-          for (int r = 0; r < 8; ++r)
-            if (j < reinterpret_cast<const int*>(pr)[(KPW + 1) * 8 + r]) {
-#pragma unroll
-              for (int y = 0; y < DV; ++y) o[r][y] = fmaf(pk[r], v[y], o[r][y]);
-            }
-        }
-      }
-    } else {
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) o[d * NT + nt][x] *= alpha[2 * nt + (x & 1)];
-      }
-      // P as the second product's B operand: keys along k, rows along n
-      uint32_t ph[NT][2], pl[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float a = s[nt][2 * e], c = s[nt][2 * e + 1];
-          const uint32_t hi = pack2_out<T>(a, c);
-          const T* const hp = reinterpret_cast<const T*>(&hi);
-          ph[nt][e] = transpose8(hi);
-          pl[nt][e] = transpose8(pack2_out<T>(a - to_float(hp[0]), c - to_float(hp[1])));
-        }
-#pragma unroll
-      for (int d0 = 0; d0 < D / 16; d0 += kAhead) {
-        if (d0 > 0) {
-#pragma unroll
-          for (int d = 0; d < kAhead; ++d) ldsm4t(va[d], vs + v_row + (((2 * (d0 + d) + ((lane >> 3) & 1)) ^ v_key) << 4));
-        }
-        bool apart = false;
-        if (apart0 < apart1) {
-#pragma unroll
-          for (int d = 0; d < kAhead; ++d)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) apart |= not_finite2<T>(va[d][x]);
-          apart = __any_sync(0xffffffffu, apart);
-        }
-        if (apart) {  // V without those keys: a register holds the lane's pair of keys, or the pair 8 on
-          const int a0 = 2 * (lane & 3);
-          const uint32_t keep0 = (a0 < apart0 ? 0xffffu : 0u) | (a0 + 1 < apart0 ? 0xffff0000u : 0u);
-          const uint32_t keep1 = (a0 + 8 < apart0 ? 0xffffu : 0u) | (a0 + 9 < apart0 ? 0xffff0000u : 0u);
-#pragma unroll
-          for (int d = 0; d < kAhead; ++d) {
-            va[d][0] &= keep0;
-            va[d][1] &= keep0;
-            va[d][2] &= keep1;
-            va[d][3] &= keep1;
-          }
-        }
-#pragma unroll
-        for (int d = 0; d < kAhead; ++d)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma<T>(o[(d0 + d) * NT + nt], va[d], ph[nt][0], ph[nt][1]);
-#pragma unroll
-        for (int d = 0; d < kAhead; ++d)
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma<T>(o[(d0 + d) * NT + nt], va[d], pl[nt][0], pl[nt][1]);
-        if (apart) {
-          for (int k = apart0; k < apart1; ++k) {
-            const int src = (k & 7) * 4 + (lane & 3);
-            const unsigned char* const row = st + (BK + key0 + k) * C::PITCH;
-            const int ck = C::key(key0 + k);
-            auto v_at = [&](int ch) { return to_float(reinterpret_cast<const T*>(row + (ch ^ ck) * 16)[lane >> 2]); };  // head dim 8 ch + lane / 4
-            const int j = b.kb * BK + key0 + k;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const float w = __shfl_sync(0xffffffffu, k < 8 ? s[nt][x] : s[nt][x + 2], src);
-                if (j < limit[2 * nt + x]) {
-#pragma unroll
-                  for (int d = d0; d < d0 + kAhead; ++d) {
-                    o[d * NT + nt][x] = fmaf(w, v_at(2 * d), o[d * NT + nt][x]);
-                    o[d * NT + nt][x + 2] = fmaf(w, v_at(2 * d + 1), o[d * NT + nt][x + 2]);
-                  }
-                }
-              }
-          }
-        }
-      }
-    }
+    BlockView view;
+    view.k = st;
+    view.v = st + BK * C::PITCH;
+    view.first = b.kb * BK;
+    view.len = b.len;
+    view.every = b.len - p.T + 1;
+    view.masked = (b.kb + 1) * BK > view.every;
+    tile.block(p, view);
 
     // ---- end of the unit, or of this CTA's part of it: the warps' sums are joined ----
     if (b.kb == nb - 1 || i == n_iter - 1) {
@@ -703,40 +332,13 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
         const long long units = ((long long)b.seq * p.H_kv + h) * p.row_tiles + (b.hr >> 16) + 1;
         p.meta[blockIdx.x] = make_int4(b.seq, b.hr, (int)((first + i - b.kb + nb - 1 + units * kUnitCost) / piece.share), b.len);
       }
-#pragma unroll
-      for (int c = 0; c < 2 * NT; ++c) {
-        l[c] += __shfl_xor_sync(0xffffffffu, l[c], 4);
-        l[c] += __shfl_xor_sync(0xffffffffu, l[c], 8);
-        l[c] += __shfl_xor_sync(0xffffffffu, l[c], 16);
-      }
-      if (lane < 4) {
-#pragma unroll
-        for (int c = 0; c < 2 * NT; ++c) join_ml[warp * C::ROWS_G + (c >> 1) * 8 + 2 * lane + (c & 1)] = make_float2(m[c], l[c]);
-      }
+      tile.stats(join_ml + warp * C::ROWS_G);
       float* const join = reinterpret_cast<float*>(st);   // once all warps are through with the block
 #pragma unroll
       for (int part = 0; part < RG * NT; ++part) {      // 8 rows of one row group at a time
         const int pg = part / NT, nt = part % NT;
         __syncthreads();
-        if (rg == pg) {
-          float* const mine = join + kw * 8 * C::MP;
-          if constexpr (kFp32) {
-            constexpr int DV = (D + 31) / 32;
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-#pragma unroll
-              for (int y = 0; y < DV; ++y) {
-                const int d = D >= 128 ? (y / 4) * 128 + lane * 4 + (y & 3) : lane * DV + y;
-                if (d < D) mine[r * C::MP + d] = o[r][y];
-              }
-          } else {
-#pragma unroll
-            for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-              for (int x = 0; x < 4; ++x)
-                mine[(2 * (lane & 3) + (x & 1)) * C::MP + d * 16 + (lane >> 2) + (x >> 1) * 8] = o[d * NT + nt][x];
-          }
-        }
+        if (rg == pg) tile.rows(join + kw * 8 * C::MP, nt);
         __syncthreads();
         constexpr int Q4 = D / 4;
         for (int e = tid; e < 8 * Q4; e += C::THREADS) {
@@ -774,68 +376,99 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
   }
 }
 
-// Joins the parts of a unit, in the order of the pieces: block (c, row) takes a row of the unit that begins in piece c and ends
-// in a later one.  Groups of D / 4 threads take the parts in turn, several loads in flight each, and are summed in their own order.
+// Joins the parts of a unit, in the order of the pieces: blocks (c, *) take the unit that begins in piece c and ends in a later one.
+// A unit of few parts is joined row by row, D / 4 threads a row; the rows of one in many pieces (few units, long ones) are each
+// joined by a whole block, whose groups of D / 4 threads take the parts in turn and are summed in their own order.
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(256) combine_kernel(const DecodeParams p) {
   constexpr int Q4 = D / 4, GROUPS = 256 / Q4;
-  constexpr int MOST = 512;                       // parts whose weights are held at a time
+  constexpr int FEW = 8, MOST = 256;              // parts that a thread takes alone; parts whose weights are held at a time
   __shared__ float wt[MOST];
   __shared__ float red[8], red_l[8];
   __shared__ float4 sums[GROUPS][Q4];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 u = p.meta[blockIdx.x];
   if (u.x < 0) return;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, group = tid / Q4, q = tid % Q4;
   const int c0 = blockIdx.x, n = u.z - c0 + 1;
-  const int h = u.y & 0xffff, rt = blockIdx.y, r = (u.y >> 16) * ROWS + rt;
-  if (r >= p.R) return;
-  auto part = [&](int c) { return (int64_t)(2 * (c0 + c) + (c == 0)) * ROWS + rt; };
+  const int h = u.y & 0xffff, row0 = (u.y >> 16) * ROWS, rows = min(ROWS, p.R - row0);
+  auto part = [&](int c, int rt) { return (int64_t)(2 * (c0 + c) + (c == 0)) * ROWS + rt; };
 
-  float all = -INFINITY;
-  for (int c = tid; c < n; c += 256) all = fmaxf(all, __ldcg(&p.part_ml[part(c)]).x);
+  if (n <= FEW) {
+    for (int rt = blockIdx.y * GROUPS + group; rt < rows; rt += gridDim.y * GROUPS) {
+      float2 ml[FEW];
+      float4 x[FEW];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
-  if ((tid & 31) == 0) red[tid >> 5] = all;
-  __syncthreads();
+      for (int c = 0; c < FEW; ++c)
+        if (c < n) {
+          ml[c] = __ldcg(&p.part_ml[part(c, rt)]);
+          x[c] = __ldcg(reinterpret_cast<const float4*>(p.part_o + part(c, rt) * D + q * 4));
+        }
+      float all = -INFINITY;
 #pragma unroll
-  for (int w = 0; w < 8; ++w) all = fmaxf(all, red[w]);
+      for (int c = 0; c < FEW; ++c)
+        if (c < n) all = fmaxf(all, ml[c].x);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float ls = 0.f;
+#pragma unroll
+      for (int c = 0; c < FEW; ++c)
+        if (c < n) {
+          const float w = weight(ml[c].x, all);   // (a part that saw nothing, or only -inf, weighs nothing)
+          ls += w * ml[c].y;
+          sum.x += w * x[c].x; sum.y += w * x[c].y; sum.z += w * x[c].z; sum.w += w * x[c].w;
+        }
+      write_row<T>(p, u.x, h, row0 + rt, u.w, D, q * 4, sum, all, ls);
+    }
+    return;
+  }
 
-  const int group = tid / Q4, q = tid % Q4;
-  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  float ls = 0.f;
-  for (int base = 0; base < n; base += MOST) {
-    const int m = min(MOST, n - base);
-    if (base > 0) __syncthreads();
-    for (int c = tid; c < m; c += 256) {
-      const float2 x = __ldcg(&p.part_ml[part(base + c)]);
-      const float w = weight(x.x, all);           // (a part that saw nothing, or only -inf, weighs nothing)
-      wt[c] = w;
-      ls += w * x.y;
+  for (int rt = blockIdx.y; rt < rows; rt += gridDim.y) {
+    float all = -INFINITY;
+    for (int c = tid; c < n; c += 256) all = fmaxf(all, __ldcg(&p.part_ml[part(c, rt)]).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, o));
+    if ((tid & 31) == 0) red[tid >> 5] = all;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 8; ++w) all = fmaxf(all, red[w]);
+
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    float ls = 0.f;
+    for (int base = 0; base < n; base += MOST) {
+      const int m = min(MOST, n - base);
+      if (base > 0) __syncthreads();
+      if (tid < m) {
+        const float2 x = __ldcg(&p.part_ml[part(base + tid, rt)]);
+        const float w = weight(x.x, all);
+        wt[tid] = w;
+        ls += w * x.y;
+      }
+      __syncthreads();
+#pragma unroll 8
+      for (int c = group; c < m; c += GROUPS) {
+        const float w = wt[c];
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + part(base + c, rt) * D + q * 4));
+        sum.x += w * x.x; sum.y += w * x.y; sum.z += w * x.z; sum.w += w * x.w;
+      }
+    }
+    sums[group][q] = sum;
+    ls = warp_sum(ls);
+    if ((tid & 31) == 0) red_l[tid >> 5] = ls;
+    __syncthreads();
+    if (tid < Q4) {
+      sum = sums[0][tid];
+#pragma unroll
+      for (int g = 1; g < GROUPS; ++g) {
+        const float4 x = sums[g][tid];
+        sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
+      }
+      ls = red_l[0];
+#pragma unroll
+      for (int w = 1; w < 8; ++w) ls += red_l[w];
+      write_row<T>(p, u.x, h, row0 + rt, u.w, D, tid * 4, sum, all, ls);
     }
     __syncthreads();
-#pragma unroll 8
-    for (int c = group; c < m; c += GROUPS) {
-      const float w = wt[c];
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + part(base + c) * D + q * 4));
-      sum.x += w * x.x; sum.y += w * x.y; sum.z += w * x.z; sum.w += w * x.w;
-    }
   }
-  sums[group][q] = sum;
-  ls = warp_sum(ls);
-  if ((tid & 31) == 0) red_l[tid >> 5] = ls;
-  __syncthreads();
-  if (tid >= Q4) return;
-  sum = sums[0][tid];
-#pragma unroll
-  for (int g = 1; g < GROUPS; ++g) {
-    const float4 x = sums[g][tid];
-    sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
-  }
-  ls = red_l[0];
-#pragma unroll
-  for (int w = 1; w < 8; ++w) ls += red_l[w];
-  write_row<T>(p, u.x, h, r, u.w, D, tid * 4, sum, all, ls);
 }
 
 // What a shape runs on: rows of a tile, CTAs, workspace.
@@ -862,7 +495,10 @@ int launch_config(const DecodeParams& p, int ctas, int min_share, bool splits, c
   if (!splits) return 0;
   LaunchScope scope(kKPagedCombine, s);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas, p.R < C::ROWS ? p.R : C::ROWS);
+  // a block for 256 x 4 values of a unit, or one for each row where units are in many parts
+  const int rows = p.R < C::ROWS ? p.R : C::ROWS;
+  const bool many = (long long)p.n_seq * p.H_kv * p.row_tiles * 6 < ctas;
+  cfg.gridDim = dim3(ctas, many ? rows : (rows * C::D / 4 + 255) / 256);
   cfg.blockDim = dim3(256);
   cfg.stream = s;
   // its blocks may be made while the kernel above still runs; they wait for its end
@@ -882,17 +518,18 @@ Plan plan_of(int R) { return Plan{C::ROWS, (R + C::ROWS - 1) / C::ROWS, C::CTAS,
 template <typename T, int D>
 Plan plan_for(int R) {
   if constexpr (sizeof(T) == 4) {
-    if (R <= 8) return plan_of<Config<T, D, 1, 1, 4>>(R);
-    return plan_of<Config<T, D, 1, 2, 4>>(R);
-  } else if constexpr (D == 256) {
-    if (R <= 8) return plan_of<Config<T, D, 1, 1, 4>>(R);
-    if (R <= 16) return plan_of<Config<T, D, 1, 2, 4>>(R);
-    return plan_of<Config<T, D, 1, 4, 4>>(R);
+    if (R <= 8) return plan_of<Config<T, D, kSingle, 1, 4, 2>>(R);
+    return plan_of<Config<T, D, kSingle, 2, 4, 2>>(R);
   } else {
-    if (R <= 8) return plan_of<Config<T, D, 1, 1, PD_KW>>(R);
-    if (R <= 16) return plan_of<Config<T, D, 2, 1, 4>>(R);
-    if (R <= 32) return plan_of<Config<T, D, 2, 2, 4>>(R);
-    return plan_of<Config<T, D, 2, 4, 4>>(R);
+    if (R <= 8) return plan_of<Config<T, D, kNarrow, 1, 4, D == 256 ? 2 : 3>>(R);
+    if constexpr (D == 256) {
+      if (R <= 16) return plan_of<Config<T, D, kNarrow, 2, 4, 1>>(R);
+      return plan_of<Config<T, D, kWide, 2, 4, 1>>(R);
+    } else {
+      if (R <= 16) return plan_of<Config<T, D, kWide, 1, 4, 3>>(R);
+      if (R <= 32) return plan_of<Config<T, D, kWide, 2, 2, D <= 64 ? 3 : 2>>(R);
+      return plan_of<Config<T, D, kWide, 4, 1, D <= 64 ? 3 : 2>>(R);
+    }
   }
 }
 
