@@ -381,12 +381,14 @@ def test_decode_what_a_row_does_not_see_does_not_reach_it(dtype, bad):
     lens = [4, 16, 17, 20, 64, 67, 130]
     kc, vc, table = paged_cache(lens, 2, D, 16, dtype, gen)
     q = _randn(gen, len(lens), T, 6, D, dtype=dtype)
-    want = vb.paged_decode_attn(q, kc, vc, page_table=table, cache_seqlens=_ints(lens))
+    # (their sums may go another way where V is not finite, so they are held to the formula like any other row, not to the bits
+    # of a call whose V is finite)
+    want, _, off, _ = decode(q, kc, vc, table, lens)
     for which in (vc, kc):
         for i, n in enumerate(lens):
             which[table[i, (n - 1) // 16].long(), (n - 1) % 16] = bad
         got = vb.paged_decode_attn(q, kc, vc, page_table=table, cache_seqlens=_ints(lens))
-        assert torch.equal(got[:, :T - 1], want[:, :T - 1])
+        assert_within(got[:, :T - 1], want[:, :T - 1], off[:, :T - 1], "rows that do not see it")
         assert not torch.isfinite(got[:, T - 1]).all(-1).any()
 
 

@@ -23,23 +23,23 @@ namespace vafa {
 namespace paged {
 
 // How a shape is cut: RG groups of KW warps, a group's warps share out the keys of a block and have ROWS_G rows each; at most MOST CTAs an SM.
-enum Kind { kNarrow, kWide, kSingle };  // (kSingle: fp32)
+enum Kind { kNarrow, kWide, kFma4, kFma8 };  // (the last two: fp32, 4 or 8 rows a warp)
 template <typename T_, int D_, Kind KIND_, int RG_, int KW_, int MOST_>
 struct Config {
   using T = T_;
   static constexpr int D = D_, RG = RG_, KW = KW_;
   static constexpr Kind KIND = KIND_;
-  static constexpr bool kFp32 = KIND == kSingle;
+  static constexpr bool kFp32 = KIND == kFma4 || KIND == kFma8;
   static_assert(kFp32 == (sizeof(T) == 4), "fp32 has a tile of its own");
   static constexpr int NT = KIND == kWide ? 2 : 1;           // groups of 8 rows of a warp
-  static constexpr int KPW = kFp32 ? (D >= 128 ? 8 : 16) : KIND == kWide ? 64 / KW : D <= 64 ? 32 : 16;  // keys of a warp
+  static constexpr int KPW = kFp32 ? (D >= 128 ? 8 : D == 64 ? 16 : 32) : KIND == kWide ? 64 / KW : D <= 64 ? 32 : 16;  // keys of a warp
   static constexpr int BK = KW * KPW;
-  static constexpr int ROWS_G = 8 * NT, ROWS = ROWS_G * RG;
+  static constexpr int ROWS_G = KIND == kFma4 ? 4 : 8 * NT, ROWS = ROWS_G * RG;
   static constexpr int THREADS = 32 * KW * RG;
   static_assert(BK <= THREADS, "a thread looks up a key's place");
   static constexpr int VEC = 16 / (int)sizeof(T), CH = D / VEC;
-  // A row's 16-byte chunks are stored at chunk ^ key(row): the 8 rows that an ldmatrix tile (fp32: the 2 rows that 8 lanes)
-  // read at the same chunk then lie in different banks without padding.
+  // A row's 16-byte chunks are stored at chunk ^ key(row): the 8 rows that an ldmatrix tile reads at the same chunk then lie in
+  // different banks without padding (fp32: so do the 64 bytes that 4 lanes read of each of two neighbouring rows).
   static constexpr int PITCH = D * (int)sizeof(T);
   static __device__ __forceinline__ int key(int row) {
     if constexpr (kFp32) return CH >= 8 ? (row & 1) * 4 : 0;
@@ -52,7 +52,7 @@ struct Config {
   static constexpr int kJoinBytes = KW * 8 * MP * 4;
   static_assert(kJoinBytes <= kStageBytes, "the join buffer takes the place of a stage that has been read");
   static constexpr int kMlBytes = RG * KW * ROWS_G * 8;
-  static constexpr int kPBytes = kFp32 ? RG * KW * (KPW + 2) * 8 * 4 : 0;
+  static constexpr int kPBytes = kFp32 ? RG * KW * (KPW + 2) * ROWS_G * 4 : 0;
   static constexpr int kBudget = 227 * 1024;
   static constexpr int kMaxStages = 6;
   static constexpr int bytes_of(int s) { return s * kStageBytes + kQBytes + kMlBytes + kPBytes + (s + 2) * (16 + BK * 16) + 256; }
@@ -312,7 +312,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
         __syncthreads();
         q = q_now;
       }
-      tile.begin(p, q, b.len, row0, p_all + warp * (C::KPW + 2) * 8);
+      tile.begin(p, q, b.len, row0, p_all + warp * (C::KPW + 2) * C::ROWS_G);
     }
     BlockView view;
     view.k = st;
@@ -518,8 +518,9 @@ Plan plan_of(int R) { return Plan{C::ROWS, (R + C::ROWS - 1) / C::ROWS, C::CTAS,
 template <typename T, int D>
 Plan plan_for(int R) {
   if constexpr (sizeof(T) == 4) {
-    if (R <= 8) return plan_of<Config<T, D, kSingle, 1, 4, 2>>(R);
-    return plan_of<Config<T, D, kSingle, 2, 4, 2>>(R);
+    if (R <= 4) return plan_of<Config<T, D, kFma4, 1, 4, 3>>(R);
+    if (R <= 8) return plan_of<Config<T, D, kFma8, 1, 4, 3>>(R);
+    return plan_of<Config<T, D, kFma8, 2, 4, 2>>(R);
   } else {
     if (R <= 8) return plan_of<Config<T, D, kNarrow, 1, 4, D == 256 ? 2 : 3>>(R);
     if constexpr (D == 256) {

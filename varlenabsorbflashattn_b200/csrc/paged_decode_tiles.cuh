@@ -7,8 +7,8 @@
 //               1/16 full; a K or V element meets 8 rows, far below any tensor limit, so that HBM bounds it.
 //   WideTile    16-bit, more rows (several tokens, many grouped heads): the query rows as the 16 rows of the product, so that P goes
 //               from one product to the next in registers and statistics are kept for 2 rows a thread instead of 4.
-//   Fp32Tile    fp32 multiply-adds (tensor products of fp32 would round to tf32): 4 lanes a key for the scores, then the
-//               head dim over the lanes for P V.
+//   Fp32Tile    fp32 multiply-adds (tensor products of fp32 would round to tf32), 4 or 8 rows: 4 lanes a key for the scores, then
+//               the head dim over the lanes for P V.
 // 16-bit P is split into two pieces (hi + lo) for the second product: one piece would put an error of the size of the output's own
 // rounding on top of it (2.4e-3 instead of 1.7e-3 of bf16 outputs); the second costs a product per V fragment and no time that shows.
 // Keys that some rows see and others do not (the new tokens themselves) are summed apart where V is not finite: 0 times a
@@ -512,84 +512,83 @@ struct WideTile {
 template <typename C>
 struct Fp32Tile {
   static constexpr int D = C::D, KPW = C::KPW, KL = KPW / 8, DV = (D + 31) / 32;
-  float o[8][DV];             // rows 0 .. 7, head dim 128 (y / 4) + 4 lane + y % 4, or DV lane + y below 128
-  float m[2], l[2];           // rows 2 (lane % 4) + {0, 1}
-  int limit[2];
+  static constexpr int NR = C::ROWS_G, RL = NR / 4;  // rows of the warp, and of a lane where statistics are kept
+  float o[NR][DV];            // rows 0 .. NR, head dim 128 (y / 4) + 4 lane + y % 4, or DV lane + y below 128
+  float m[RL], l[RL];         // rows RL (lane % 4) .. + RL
+  int limit[RL];
   const unsigned char* q_at;
-  float* pr;                  // the warp's P [KPW][8], then alpha and the limits of the 8 rows
+  float* pr;                  // the warp's P [KPW][NR], then alpha and the limits of the rows
   int lane, key0, rg;
 
   __device__ __forceinline__ explicit Fp32Tile(const Place& w) : lane(w.lane), key0(w.kw * KPW), rg(w.rg) {}
 
   __device__ __forceinline__ void begin(const DecodeParams& p, const unsigned char* q, int len, int row0, float* scratch) {
-    q_at = q + rg * 8 * C::PITCH;
+    q_at = q + rg * NR * C::PITCH;
     pr = scratch;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < RL; ++x) {
       m[x] = -INFINITY;
       l[x] = 0.f;
-      limit[x] = row_limit(p, len, row0 + rg * 8 + 2 * (lane & 3) + x);
+      limit[x] = row_limit(p, len, row0 + rg * NR + RL * (lane & 3) + x);
     }
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int y = 0; y < DV; ++y) o[r][y] = 0.f;
   }
 
   __device__ __forceinline__ void block(const DecodeParams& p, const BlockView& b) {
-    float s[4];  // key lane / 4 (+ 8 for x >= 2), rows 2 (lane % 4) + {0, 1}
-    float acc[KL][8];
+    float s[KL][RL];  // key 8 e + lane / 4, the lane's rows
+    {
+      float acc[KL][NR];
 #pragma unroll
-    for (int e = 0; e < KL; ++e)
+      for (int e = 0; e < KL; ++e)
 #pragma unroll
-      for (int r = 0; r < 8; ++r) acc[e][r] = 0.f;
-    const unsigned char* const kr = b.k + (key0 + (lane >> 2)) * C::PITCH;  // (keys 8 apart have the same key())
-    const unsigned char* const qr = q_at;
-    const int ck = C::key(lane >> 2);
+        for (int r = 0; r < NR; ++r) acc[e][r] = 0.f;
+      const unsigned char* const kr = b.k + (key0 + (lane >> 2)) * C::PITCH;  // (keys 8 apart have the same key())
+      const int ck = C::key(lane >> 2);
 #pragma unroll 4
-    for (int d = 0; d < D / 16; ++d) {
-      float4 kv[KL];
+      for (int d = 0; d < D / 16; ++d) {
+        float4 kv[KL];
 #pragma unroll
-      for (int e = 0; e < KL; ++e) kv[e] = *reinterpret_cast<const float4*>(kr + e * 8 * C::PITCH + ((4 * d + (lane & 3)) ^ ck) * 16);
+        for (int e = 0; e < KL; ++e) kv[e] = *reinterpret_cast<const float4*>(kr + e * 8 * C::PITCH + ((4 * d + (lane & 3)) ^ ck) * 16);
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const float4 qv = *reinterpret_cast<const float4*>(qr + r * C::PITCH + ((4 * d + (lane & 3)) ^ C::key(r)) * 16);
+        for (int r = 0; r < NR; ++r) {
+          const float4 qv = *reinterpret_cast<const float4*>(q_at + r * C::PITCH + ((4 * d + (lane & 3)) ^ C::key(r)) * 16);
 #pragma unroll
-        for (int e = 0; e < KL; ++e)
-          acc[e][r] = fmaf(qv.x, kv[e].x, fmaf(qv.y, kv[e].y, fmaf(qv.z, kv[e].z, fmaf(qv.w, kv[e].w, acc[e][r]))));
+          for (int e = 0; e < KL; ++e)
+            acc[e][r] = fmaf(qv.x, kv[e].x, fmaf(qv.y, kv[e].y, fmaf(qv.z, kv[e].z, fmaf(qv.w, kv[e].w, acc[e][r]))));
+        }
       }
-    }
-    // the four lanes of a key sum their quarters; lane % 4 keeps rows 2 (lane % 4) and the next
-#pragma unroll
-    for (int e = 0; e < KL; ++e) {
-      float h4[4];
+      // the four lanes of a key sum their quarters and share out the rows
       const bool hi2 = (lane & 2) != 0, hi1 = (lane & 1) != 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float give = hi2 ? acc[e][r] : acc[e][r + 4], keep = hi2 ? acc[e][r + 4] : acc[e][r];
-        h4[r] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
-      }
+      for (int e = 0; e < KL; ++e) {
+        float half[NR / 2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float give = hi1 ? h4[r] : h4[r + 2], keep = hi1 ? h4[r + 2] : h4[r];
-        s[2 * e + r] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+        for (int r = 0; r < NR / 2; ++r) {
+          const float give = hi2 ? acc[e][r] : acc[e][r + NR / 2], keep = hi2 ? acc[e][r + NR / 2] : acc[e][r];
+          half[r] = keep + __shfl_xor_sync(0xffffffffu, give, 2);
+        }
+#pragma unroll
+        for (int r = 0; r < RL; ++r) {
+          const float give = hi1 ? half[r] : half[r + RL], keep = hi1 ? half[r + RL] : half[r];
+          s[e][r] = keep + __shfl_xor_sync(0xffffffffu, give, 1);
+        }
       }
     }
     const int j0 = b.first + key0 + (lane >> 2);
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      if (x >= 2 * KL) {
-        s[x] = -INFINITY;
-        continue;
-      }
-      s[x] *= p.scale_log2;
-      if (b.masked && (j0 + (x >> 1) * 8 >= limit[x & 1])) s[x] = -INFINITY;
-    }
-    float alpha[2];
+    float alpha[RL];
     bool moved = false;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      float top = fmaxf(s[x], s[x + 2]);
+    for (int x = 0; x < RL; ++x) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < KL; ++e) {
+        s[e][x] *= p.scale_log2;
+        if (b.masked && (j0 + 8 * e >= limit[x])) s[e][x] = -INFINITY;
+        top = fmaxf(top, s[e][x]);
+      }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -597,25 +596,31 @@ struct Fp32Tile {
       moved |= now != m[x];
       alpha[x] = weight(m[x], now);
       const float ref = now == -INFINITY ? 0.f : now;
-      s[x] = exp2_approx(s[x] - ref);
-      s[x + 2] = exp2_approx(s[x + 2] - ref);
-      l[x] = l[x] * alpha[x] + (s[x] + s[x + 2]);
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < KL; ++e) {
+        s[e][x] = exp2_approx(s[e][x] - ref);
+        sum += s[e][x];
+      }
+      l[x] = l[x] * alpha[x] + sum;
       m[x] = now;
     }
     const int apart0 = p.T > 1 && b.masked ? max(0, b.every - (b.first + key0)) : KPW;
     __syncwarp();
 #pragma unroll
-    for (int e = 0; e < KL; ++e)
-      *reinterpret_cast<float2*>(pr + (8 * e + (lane >> 2)) * 8 + 2 * (lane & 3)) = make_float2(s[2 * e], s[2 * e + 1]);
-    if (lane < 4) {
-      *reinterpret_cast<float2*>(pr + KPW * 8 + 2 * lane) = make_float2(alpha[0], alpha[1]);
-      *reinterpret_cast<int2*>(pr + (KPW + 1) * 8 + 2 * lane) = make_int2(limit[0], limit[1]);
+    for (int x = 0; x < RL; ++x) {
+#pragma unroll
+      for (int e = 0; e < KL; ++e) pr[(8 * e + (lane >> 2)) * NR + RL * (lane & 3) + x] = s[e][x];
+      if (lane < 4) {
+        pr[KPW * NR + RL * lane + x] = alpha[x];
+        reinterpret_cast<int*>(pr)[(KPW + 1) * NR + RL * lane + x] = limit[x];
+      }
     }
     __syncwarp();
     if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r) {
-        const float f = pr[KPW * 8 + r];
+      for (int r = 0; r < NR; ++r) {
+        const float f = pr[KPW * NR + r];
 #pragma unroll
         for (int y = 0; y < DV; ++y) o[r][y] *= f;
       }
@@ -625,8 +630,12 @@ struct Fp32Tile {
     const bool has = D >= 32 || lane < D;
 #pragma unroll 4
     for (int k = 0; k < KPW; ++k) {
-      const float4 pa = *reinterpret_cast<const float4*>(pr + k * 8), pb = *reinterpret_cast<const float4*>(pr + k * 8 + 4);
-      const float pk[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
+      float pk[NR];
+#pragma unroll
+      for (int r = 0; r < NR; r += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(pr + k * NR + r);
+        pk[r] = x.x; pk[r + 1] = x.y; pk[r + 2] = x.z; pk[r + 3] = x.w;
+      }
       float v[DV];
       const unsigned char* const row = vr + k * C::PITCH;
       const int ck = C::key(k);
@@ -646,14 +655,14 @@ struct Fp32Tile {
       }
       if (k < apart0) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
           for (int y = 0; y < DV; ++y) o[r][y] = fmaf(pk[r], v[y], o[r][y]);
       } else {
         const int j = b.first + key0 + k;
 #pragma unroll
-        for (int r = 0; r < 8; ++r)
-          if (j < reinterpret_cast<const int*>(pr)[(KPW + 1) * 8 + r]) {
+        for (int r = 0; r < NR; ++r)
+          if (j < reinterpret_cast<const int*>(pr)[(KPW + 1) * NR + r]) {
 #pragma unroll
             for (int y = 0; y < DV; ++y) o[r][y] = fmaf(pk[r], v[y], o[r][y]);
           }
@@ -663,16 +672,16 @@ struct Fp32Tile {
 
   __device__ __forceinline__ void stats(float2* out) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < RL; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 4);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 8);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 16);
-      if (lane < 4) out[2 * lane + x] = make_float2(m[x], l[x]);
+      if (lane < 4) out[RL * lane + x] = make_float2(m[x], l[x]);
     }
   }
   __device__ __forceinline__ void rows(float* out, int) const {
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
+    for (int r = 0; r < NR; ++r)
 #pragma unroll
       for (int y = 0; y < DV; ++y) {
         const int d = D >= 128 ? (y / 4) * 128 + lane * 4 + (y & 3) : lane * DV + y;
