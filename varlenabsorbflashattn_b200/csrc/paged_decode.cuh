@@ -38,6 +38,7 @@ struct Config {
   static constexpr int THREADS = 32 * KW * RG;
   static_assert(BK <= THREADS, "a thread looks up a key's place");
   static constexpr int VEC = 16 / (int)sizeof(T), CH = D / VEC;
+  static_assert(THREADS % CH == 0, "a thread copies the same chunk of all its rows");
   // A row's 16-byte chunks are stored at chunk ^ key(row): the 8 rows that an ldmatrix tile reads at the same chunk then lie in
   // different banks without padding (fp32: so do the 64 bytes that 4 lanes read of each of two neighbouring rows).
   static constexpr int PITCH = D * (int)sizeof(T);
@@ -164,6 +165,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
   constexpr int D = C::D, NT = C::NT, RG = C::RG, BK = C::BK, KW = C::KW, S = C::S;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Piece piece;
+  __shared__ volatile int missing;     // a page outside the cache has been met
   __shared__ long long scan[C::THREADS / 32];
 
   unsigned char* const stages = smem;
@@ -179,6 +181,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
   const int kw = warp % KW, rg = warp / KW;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 0) missing = 0;
   find_piece<C>(p, &piece, scan, min_share);
   const long long first = piece.first;
   const int n_iter = (int)(piece.last - first);
@@ -219,38 +222,52 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
       }
     }
   };
+  // a key's place in bytes from the head's first element; 0 for what lies behind the sequence, -1 for a page that is not there
   auto land = [&](const Lookup& x, int i) {
     const int slot = i % C::kInfo;
     if (tid == 0) info[slot] = x.b;
-    longlong2 r = make_longlong2(-1, -1);
+    longlong2 r = make_longlong2(0, 0);
     if (x.b.seq < p.n_seq && x.b.kb * BK + tid < x.b.len) {
-      if (x.page >= 0 && x.page < p.num_pages)
-        r = make_longlong2(x.page * p.k_page + x.slot * p.k_slot, x.page * p.v_page + x.slot * p.v_slot);
-      else
+      if (x.page >= 0 && x.page < p.num_pages) {
+        r = make_longlong2((x.page * p.k_page + x.slot * p.k_slot) * (int)sizeof(T), (x.page * p.v_page + x.slot * p.v_slot) * (int)sizeof(T));
+      } else {
+        r = make_longlong2(-1, -1);
+        missing = 1;
         report_error(p.status, kBadCacheIndex, kSiteDecode, x.b.seq);
+      }
     }
     row_at[slot * BK + tid] = r;
   };
   // copies block i (of this CTA) into its stage
   auto issue = [&](int i) {
     const Block b = info[i % C::kInfo];
-    const longlong2* const rows = row_at + (i % C::kInfo) * BK;
+    const longlong2* const rows = row_at + (i % C::kInfo) * BK + tid / C::CH;
     const int h = b.hr & 0xffff;
     unsigned char* const st = stages + (i % S) * C::kStageBytes;
-    const T* const kh = reinterpret_cast<const T*>(p.k) + h * p.k_head;
-    const T* const vh = reinterpret_cast<const T*>(p.v) + h * p.v_head;
+    const char* const kh = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + h * p.k_head) + tid % C::CH * 16;
+    const char* const vh = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + h * p.v_head) + tid % C::CH * 16;
     const uint32_t ks = smem_addr(st), vs = ks + BK * C::PITCH, qs = vs + BK * C::PITCH;
+    constexpr int kRows = C::THREADS / C::CH;             // rows of a step: a thread has the same chunk of each of its rows
+    const int here = b.len - b.kb * BK;                   // keys of the block
+    auto copy = [&](auto all) {
 #pragma unroll
-    for (int x = 0; x < (BK * C::CH + C::THREADS - 1) / C::THREADS; ++x) {
-      const int e = x * C::THREADS + tid;
-      if ((BK * C::CH) % C::THREADS != 0 && e >= BK * C::CH) break;
-      const int row = e / C::CH, ch = e % C::CH;
-      const longlong2 r = rows[row];
-      const bool real = r.x >= 0;
-      const int to = row * C::PITCH + (ch ^ C::key(row)) * 16;
-      copy16(ks + to, kh + (real ? r.x + ch * C::VEC : 0), real);
-      copy16(vs + to, vh + (real ? r.y + ch * C::VEC : 0), real);
-    }
+      for (int x = 0; x < (BK + kRows - 1) / kRows; ++x) {
+        const int row = x * kRows + tid / C::CH;
+        if (BK % kRows != 0 && row >= BK) break;
+        const longlong2 r = rows[x * kRows];
+        const int to = row * C::PITCH + ((tid % C::CH) ^ C::key(row)) * 16;
+        if (decltype(all)::value) {
+          copy16(ks + to, kh + r.x, true);
+          copy16(vs + to, vh + r.y, true);
+        } else {  // zeros behind the sequence, and for pages that are not there
+          const bool real = row < here && r.x >= 0;
+          copy16(ks + to, kh + (real ? r.x : 0), real);
+          copy16(vs + to, vh + (real ? r.y : 0), real);
+        }
+      }
+    };
+    if (here >= BK && !missing) copy(std::true_type{});
+    else copy(std::false_type{});
     if (i == 0 || b.kb == 0) {
       const int row0 = (b.hr >> 16) * C::ROWS;
       const T* const qb = reinterpret_cast<const T*>(p.q) + b.seq * p.q_seq;
