@@ -139,6 +139,8 @@ def test_rotary_refusals():
         rot(q, k, cos, sin, cu_seqlens=_cu([1, 5]))
     with pytest.raises(ValueError, match="leave the table"):
         rot(q, k, cos, sin, positions=torch.tensor([0, 1, 2, 3, -1, 0]))
+    with pytest.raises(ValueError, match="leave the table"):
+        rot(q, k, cos, sin, positions=torch.tensor([0, 1, 2, 3, 2**32, 0]))  # 0 in 32 bits
     with pytest.raises(ValueError, match="one of"):
         rot(q, k, cos, sin)
     with pytest.raises(ValueError, match="one of"):
@@ -270,6 +272,21 @@ def test_append_passes_over_padding_and_what_is_out_of_range(unchecked):
     assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
 
 
+def test_append_is_an_operation_in_place():
+    """Autograd notices that a cache it has kept for a gradient was written to."""
+    gen = _gen(22)
+    kc, vc, table = paged_cache([8, 8], 2, 64, 4, F32, gen, fill=0.0)
+    k, w = _randn(gen, 2, 2, 64), torch.ones((), device="cuda", requires_grad=True)
+    y = (w * kc).sum()
+    vb.paged_kv_append(k, k, kc, vc, page_table=table, cache_seqlens=_ints([8, 8]))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        kc, vc = kc.clone(), vc.clone()
+        vb.paged_kv_append(k, k, kc, vc, page_table=table, cache_seqlens=_ints([5, 6]))
+        vb.paged_decode_attn(k, kc, vc, page_table=table, cache_seqlens=_ints([5, 6]))
+
+
 def test_append_refusals():
     gen = _gen(10)
     kc, vc, table = paged_cache([8, 8], 2, 64, 4, BF16, gen, fill=0.0)
@@ -283,6 +300,7 @@ def test_append_refusals():
             ("leaves the table", ValueError, lambda: call(k, v, kc, vc, cos=cos[:7], sin=sin[:7])),
             ("cache_seqlens", ValueError, lambda: call(k, v, kc, vc, cache_seqlens=_ints([8, 13]))),
             ("outside", ValueError, lambda: call(k, v, kc, vc, page_table=table + 50)),
+            ("outside", ValueError, lambda: call(k, v, kc, vc, page_table=table.long() - 2**32)),
             ("go together", ValueError, lambda: call(k, v, kc, vc, cos=cos)),
             ("without them", ValueError, lambda: call(k, v, kc, vc, q=q)),
             ("need cu_seqlens", AssertionError, lambda: call(k[:1], v[:1], kc, vc)),
@@ -452,6 +470,8 @@ def test_decode_refusals():
     for match, error, f in [
             ("cache_seqlens", ValueError, lambda: call(cache_seqlens=_ints([8, 13]))),
             ("cache_seqlens", ValueError, lambda: call(cache_seqlens=_ints([8, -1]))),
+            ("cache_seqlens", ValueError, lambda: call(cache_seqlens=torch.tensor([8, 2**32 + 8]))),
+            ("outside", ValueError, lambda: call(page_table=table.long() + 2**32)),
             ("outside", ValueError, lambda: call(page_table=table + 50)),
             ("1-D", ValueError, lambda: call(cache_seqlens=lens[None])),
             ("2-D", ValueError, lambda: call(page_table=table[0])),

@@ -38,7 +38,7 @@ int check_decode(const vafa_paged_attn_args* a) {
   if (!dim_ok(a->head_dim)) return fail(VAFA_ERR_UNSUPPORTED, "head_dim %d not supported (16/32/64/128/256)", a->head_dim);
   if (a->q_len < 1 || a->num_heads < 1 || a->num_kv_heads < 1 || a->num_heads % a->num_kv_heads)
     return fail(VAFA_ERR_INVALID, "bad sizes q_len=%d H=%d H_kv=%d (H_kv must divide H)", a->q_len, a->num_heads, a->num_kv_heads);
-  if ((long long)a->q_len * a->num_heads > (1 << 20) || a->num_kv_heads > 0xffff) return fail(VAFA_ERR_UNSUPPORTED, "q_len %d x %d heads", a->q_len, a->num_heads);
+  if ((long long)a->q_len * a->num_heads > (1 << 18) || a->num_kv_heads > 0xffff) return fail(VAFA_ERR_UNSUPPORTED, "q_len %d x %d heads", a->q_len, a->num_heads);
   return check_cache(a->n_seq, a->num_pages, a->page_size, a->max_pages);
 }
 

@@ -289,6 +289,7 @@ def packed_rotary(
         cu_seqlens, seqinfo = _lengths_to_cu(seqinfo), None
     key = ("packed_rotary", _layout(q), _layout(k), _layout(cos), _layout(sin), _layout(cu_seqlens), _layout(positions), seqinfo is None, interleaved)
     plan = _plans.get(key)
+    given = cu_seqlens if positions is None else positions  # (before it is taken to 32 bits)
     q4 = k4 = False
     if plan is None:
         q, q4 = _rows(q, "q")
@@ -314,7 +315,7 @@ def packed_rotary(
             _keep(key, plan)
     T = q.shape[0]
     if _varlen._validate and T > 0:
-        host = _host(cu_seqlens if positions is None else positions)
+        host = _host(given)
         if positions is None:
             _check_cu(host, T, "cu_seqlens")
             low, high = 0, int((host[1:] - host[:-1]).max()) - 1
@@ -387,6 +388,7 @@ def paged_kv_append(
     tensors = (k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens, q, cos, sin)
     key = ("paged_kv_append", *map(_layout, tensors), interleaved)
     plan = _plans.get(key)
+    given = cache_seqlens, page_table, cu_seqlens  # (before they are taken to 32 bits)
     q4 = False
     if plan is None:
         k, _ = _rows(k, "k")
@@ -437,8 +439,8 @@ def paged_kv_append(
     qo = None if q is None else q.new_empty(shape)
     if T > 0 and n_seq > 0:
         if _varlen._validate:
-            _check_append(_host(cache_seqlens), _host(page_table), None if cu_seqlens is None else _host(cu_seqlens), T, k_cache.shape[0],
-                          k_cache.shape[1], None if cos is None else cos.shape[0])
+            _check_append(*(None if x is None else _host(x) for x in given), T, k_cache.shape[0], k_cache.shape[1],
+                          None if cos is None else cos.shape[0])
         a = plan.args()
         a.k, a.v, a.k_cache, a.v_cache = k.data_ptr(), v.data_ptr(), kc, vc
         a.cache_seqlens, a.page_table = cache_seqlens.data_ptr(), page_table.data_ptr()
@@ -449,6 +451,8 @@ def paged_kv_append(
         if q is not None:
             a.q, a.q_out = q.data_ptr(), qo.data_ptr()
         plan.run(a, "vafa_paged_append")
+        if not k_cache.is_inference():  # autograd is told, as by every operation in place
+            torch.autograd.graph.increment_version((k_cache, v_cache))
     elif qo is not None:
         qo.zero_()
     return qo.unsqueeze(0) if q4 else qo
@@ -461,6 +465,7 @@ def _decode(q, k_cache, v_cache, page_table, cache_seqlens, scale, with_lse):
     tensors = (q, k_cache, v_cache, page_table, cache_seqlens)
     key = ("paged_decode_attn", *map(_layout, tensors), scale)
     plan = _plans.get(key)
+    given = cache_seqlens, page_table  # (before they are taken to 32 bits)
     if plan is None:
         if q.dim() not in (3, 4):
             raise ValueError(f"q: expected [n_seq,H,D] or [n_seq,T,H,D], got {q.dim()}-D")
@@ -495,13 +500,13 @@ def _decode(q, k_cache, v_cache, page_table, cache_seqlens, scale, with_lse):
     if (kc | vc) & 15:
         raise ValueError("k_cache, v_cache: base and strides must be multiples of 16 bytes")
     if qp & 15:
-        return _decode(q.clone(), k_cache, v_cache, page_table, cache_seqlens, scale, with_lse)
+        return _decode(q.clone(), k_cache, v_cache, *reversed(given), scale, with_lse)
     o = q.new_empty(q.shape)
     lse = torch.empty(plan.out[0], dtype=torch.float32, device=plan.device) if with_lse else None
     if plan.out[1] == 0:
         return o, lse
     if _varlen._validate:
-        _check_pages(_host(cache_seqlens), _host(page_table), k_cache.shape[0], k_cache.shape[1])
+        _check_pages(*map(_host, given), k_cache.shape[0], k_cache.shape[1])
     a = plan.args()
     a.q, a.k_cache, a.v_cache, a.o = qp, kc, vc, o.data_ptr()
     a.cache_seqlens, a.page_table = cache_seqlens.data_ptr(), page_table.data_ptr()
