@@ -13,6 +13,8 @@
 //    be of any size and end inside a block; page ids are read two blocks before they are needed.
 //  - each warp has its own keys of a block with its own maximum and sum (paged_decode_tiles.cuh), so that the loop has no exchange
 //    between warps; they are joined once, at the unit's end.
+// Measured: 128 caches of 8k to 32k keys, 8 heads of 128 in bf16 (10 GB) 1.41 to 1.50 ms, 6.7 to 7.1 TB/s (a copy moves 6.56); 64 caches of
+// 1k to 16k keys, 32 query and 8 K/V heads (1.7 GB) 0.25 ms; 8 caches of up to 3k keys (59 MB) 18.5 us, 9 of them reading.
 #pragma once
 #include <atomic>
 
@@ -74,6 +76,7 @@ struct Config {
 // A piece of the line of blocks: what a CTA needs to know to find its first block.  A unit costs more than its blocks (its
 // queries, the join of the warps, the rows' way out), so the line that is cut has `kUnitCost` slots more in front of each
 // unit's blocks; a piece that begins or ends among those begins or ends with the unit's first block.
+// (32 caches of 7 to 7.2k keys, four tokens of 32 heads, 0 | 1 | 2 | 4 slots: 94 | 67 | 59 | 58 us; level on batches of one length)
 constexpr int kUnitCost = 2;
 struct Piece {
   long long first, last;      // blocks [first, last), the slots not counted
@@ -92,7 +95,7 @@ __device__ __forceinline__ int blocks_of(int len) { return len <= 0 ? 1 : (len +
 // Cuts the line.  Every thread takes a run of sequences; a scan of the runs' sums, and the threads whose runs hold the two ends
 // of the piece look for them.
 template <typename C>
-__device__ void find_piece(const DecodeParams& p, Piece* out, long long* scan, int min_share) {
+__device__ void find_piece(const DecodeParams& p, Piece* out, long long* scan) {
   constexpr int kWarps = C::THREADS / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int each = (p.n_seq + C::THREADS - 1) / C::THREADS;
@@ -121,7 +124,6 @@ __device__ void find_piece(const DecodeParams& p, Piece* out, long long* scan, i
   total *= per_seq;
   // (as many slots as 32 bits hold are cut with a short division)
   long long share = total < 0x7fffffff ? ((uint32_t)total + gridDim.x - 1) / gridDim.x : (total + gridDim.x - 1) / gridDim.x;
-  if (share < min_share) share = min_share;
 #pragma unroll
   for (int end = 0; end < 2; ++end) {
     const long long target = min(total, (blockIdx.x + end) * share);
@@ -160,7 +162,7 @@ struct Block {  // a block of the line, as its ring slot describes it
 };
 
 template <typename C>
-__global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const DecodeParams p, int min_share) {
+__global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const DecodeParams p) {
   using T = typename C::T;
   constexpr int D = C::D, NT = C::NT, RG = C::RG, BK = C::BK, KW = C::KW, S = C::S;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) missing = 0;
-  find_piece<C>(p, &piece, scan, min_share);
+  find_piece<C>(p, &piece, scan);
   const long long first = piece.first;
   const int n_iter = (int)(piece.last - first);
   if (tid == 0) p.meta[blockIdx.x] = make_int4(-1, 0, 0, 0);
@@ -491,11 +493,11 @@ __global__ void __launch_bounds__(256) combine_kernel(const DecodeParams p) {
 // What a shape runs on: rows of a tile, CTAs, workspace.
 struct Plan {
   int rows, row_tiles, ctas_per_sm, bk;
-  int (*launch)(const DecodeParams&, int ctas, int min_share, bool splits, cudaStream_t);
+  int (*launch)(const DecodeParams&, int ctas, bool splits, cudaStream_t);
 };
 
 template <typename C>
-int launch_config(const DecodeParams& p, int ctas, int min_share, bool splits, cudaStream_t s) {
+int launch_config(const DecodeParams& p, int ctas, bool splits, cudaStream_t s) {
   static std::atomic<unsigned long long> set{0};  // a bit for each device
   int dev = 0;
   VAFA_CUDA_CHECK(cudaGetDevice(&dev));
@@ -506,7 +508,7 @@ int launch_config(const DecodeParams& p, int ctas, int min_share, bool splits, c
   }
   {
     LaunchScope scope(kKPagedDecode, s);
-    decode_kernel<C><<<ctas, C::THREADS, C::kSmem, s>>>(p, min_share);
+    decode_kernel<C><<<ctas, C::THREADS, C::kSmem, s>>>(p);
     VAFA_LAUNCH_CHECK("paged_decode_kernel");
   }
   if (!splits) return 0;
@@ -531,7 +533,14 @@ int launch_config(const DecodeParams& p, int ctas, int min_share, bool splits, c
 template <typename C>
 Plan plan_of(int R) { return Plan{C::ROWS, (R + C::ROWS - 1) / C::ROWS, C::CTAS, C::BK, launch_config<C>}; }
 
-// The tile of a shape: the fewest rows that hold the unit's, up to what the registers allow.
+// The tile of a shape, by the rows of its units and the head dim.  What decides is how many warps there are to hide latencies, then how
+// often an SM reads a block from shared memory.  64 caches of 4k to 8k keys with 8 K/V heads of 128, us:
+//   up to 8 rows     narrow; 1 | 2 | 3 CTAs an SM (128 caches of 8k to 32k keys) 2782 | 1585 | 1427
+//   up to 16         wide, 4 warps on a block, 2 CTAs: 275; with one 442; two warps on a block 351; narrow with two column tiles 292
+//   up to 32         wide, 2 row groups of 2 warps, 2 CTAs: 361; one CTA 592; 2 groups of 4 warps 441; one warp a group 532
+//   up to 64         wide, 4 row groups of 1 warp, 2 CTAs: 534; of 2 warps, one CTA 636; of 4 warps 1165
+//   heads of 256     O takes twice the registers: narrow with two row groups to 16 rows, 284 (wide 376), wide beyond
+//   fp32             4 rows a warp where units have no more, 3 CTAs: 523; 8 rows 877 (two groups of 4: 851, but no gain with more rows)
 template <typename T, int D>
 Plan plan_for(int R) {
   if constexpr (sizeof(T) == 4) {
