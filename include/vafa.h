@@ -1,6 +1,6 @@
 /*
- * vafa.h -- C ABI of libvafa_b200.so: packed variable-length attention and absorbed
- * target attention for NVIDIA B200 (sm_100a).
+ * vafa.h -- C ABI of libvafa_b200.so: packed variable-length attention, absorbed
+ * target attention, and rotation, paged cache and decode beside them, for NVIDIA B200 (sm_100a).
  *
  * Every entry point takes plain pointers and sizes, enqueues its kernels on the CUDA
  * stream it is given and returns immediately: 0 on success, a negative VAFA_ERR_* code

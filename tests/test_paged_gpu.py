@@ -445,6 +445,21 @@ def test_decode_offsets_past_32_bits():
     _check_decode(q, kc, vc, table, lens)
 
 
+def test_sequences_that_share_a_prefix():
+    """Pages that are only read may be anybody's: a common prefix, a sequence twice, more of the cache than its lengths reach."""
+    gen, page = _gen(23), 16
+    kc, vc, table = paged_cache([64, 64, 64], 2, 64, page, BF16, gen)
+    table[1, :3] = table[0, :3]
+    table[2] = table[0]
+    lens = [50, 61, 50]
+    q, k, v = (_randn(gen, 3, h, 64, dtype=BF16) for h in (6, 2, 2))
+    q[2] = q[0]
+    vb.paged_kv_append(k[:2], v[:2], kc, vc, page_table=table[:2], cache_seqlens=_ints(lens[:2]))
+    with pytest.raises(ValueError, match="same slot"):
+        vb.paged_kv_append(k, v, kc, vc, page_table=table, cache_seqlens=_ints(lens))
+    _check_decode(q, kc, vc, table, lens)
+
+
 def test_decode_unchecked_pages_and_lengths(unchecked):
     """What is out of range is not followed: no fault, the status word tells, and the other sequences are right."""
     gen, lens = _gen(16), [40, 100, 33]
@@ -460,6 +475,24 @@ def test_decode_unchecked_pages_and_lengths(unchecked):
         assert _status() == [4, 912] and torch.equal(got[[0, 2]], want[[0, 2]])
     got = vb.paged_decode_attn(q, kc, vc, page_table=table, cache_seqlens=_ints([40, -5, 33]))
     assert torch.equal(got[[0, 2]], want[[0, 2]]) and (got[1] == 0).all() and _status() == [4, 912]
+
+
+def test_errors_found_on_the_device_can_be_raised(unchecked):
+    gen = _gen(24)
+    kc, vc, table = paged_cache([8, 8], 2, 64, 4, BF16, gen, fill=0.0)
+    q, lens, bad = _randn(gen, 2, 2, 64, dtype=BF16), _ints([8, 8]), table + 99
+    cos, sin = vb.rotary_table(3, 64, device="cuda")
+    _status()
+    _lib.set_check_status(True)
+    try:
+        for f in (lambda: vb.paged_decode_attn(q, kc, vc, page_table=bad, cache_seqlens=lens),
+                  lambda: vb.paged_kv_append(q, q, kc, vc, page_table=bad, cache_seqlens=lens),
+                  lambda: vb.packed_rotary(q, None, cos, sin, positions=_ints([2, 3]))):
+            with pytest.raises(RuntimeError, match="outside its array"):
+                f()
+        vb.paged_decode_attn(q, kc, vc, page_table=table, cache_seqlens=lens)
+    finally:
+        _lib.set_check_status(False)
 
 
 def test_decode_refusals():
@@ -679,3 +712,41 @@ def test_long_batches_with_rows_behind_padding_and_bad_places(unchecked):
     seq = torch.repeat_interleave(torch.arange(3), torch.tensor(lens)).cuda()
     want = _append_ref(b[:4100][keep], v[:4100][keep], *before, table, pos[keep], seq[keep], 16)
     assert torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+
+
+def test_threads_on_streams_of_their_own(unchecked):
+    """Two threads append and attend on streams of their own, layouts that no call has checked yet among them."""
+    import threading
+    cases = []
+    for seed, (n, H, H_kv, page) in enumerate([(5, 9, 3, 24), (130, 8, 1, 8)]):
+        gen, lens = _gen(40 + seed), [1 + (37 * i) % 300 for i in range(n)]
+        kc, vc, table = paged_cache(lens, H_kv, 64, page, BF16, gen, fill=0.0)
+        q, k, v = (_randn(gen, n, h, 64, dtype=BF16) for h in (H, H_kv, H_kv))
+        cases.append((q, k, v, kc, vc, table, lens, vb.rotary_table(301, 64, device="cuda")))
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            q, k, v, kc, vc, table, lens, (cos, sin) = cases[i]
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                held = _ints(lens)
+                for _ in range(30):
+                    a = vb.paged_kv_append(k, v, kc, vc, page_table=table, cache_seqlens=held, q=q, cos=cos, sin=sin)
+                    o = vb.paged_decode_attn_with_lse(a, kc, vc, page_table=table, cache_seqlens=held)
+                stream.synchronize()
+            got[i] = a, *o
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for (q, k, v, kc, vc, table, lens, _), (a, o, lse) in zip(cases, got):
+        ro, rl, eo, el = decode(a.unsqueeze(1), kc, vc, table, lens)
+        assert_within(o.unsqueeze(1), ro, eo, "o")
+        assert_within(lse.unsqueeze(1), rl, el, "lse")

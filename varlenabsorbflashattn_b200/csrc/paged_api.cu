@@ -62,9 +62,9 @@ int cut_for(const vafa_paged_attn_args* a, const paged::Plan& plan, Cut* c) {
     VAFA_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
   }
   const long long per_unit = ((long long)a->max_pages * a->page_size + plan.bk - 1) / plan.bk;
-  const long long per_seq = (long long)a->num_kv_heads * plan.row_tiles * per_unit;
-  if (per_seq > 0x7fffffffLL) return fail(VAFA_ERR_UNSUPPORTED, "a sequence has too many heads and keys");
-  const long long most = per_seq * a->n_seq;
+  const long long units = (long long)a->num_kv_heads * plan.row_tiles;
+  if (units * (per_unit + paged::kUnitCost) > 0x7fffffffLL) return fail(VAFA_ERR_UNSUPPORTED, "a sequence has too many heads and keys");
+  const long long most = units * per_unit * a->n_seq;
   // a CTA for every block until the SMs are full (pieces of at least 1 | 2 | 4 | 8 slots, one cache of 512 keys: 8.6 | 9.6 | 11.3 | 13.9 us)
   c->ctas = (int)(most < (long long)sms * plan.ctas_per_sm ? most : (long long)sms * plan.ctas_per_sm);
   c->splits = per_unit > 1;

@@ -17,6 +17,9 @@ of one tensor, or a transposed view of [num_pages, H_kv, page_size, D]).  Token 
 j % page_size of page page_table[s, j // page_size].  `cache_seqlens` counts the tokens of a sequence with the new ones
 among them, in both calls; a sequence of length 0 is padding, which is neither written nor attended over.
 
+The first call on a device is made outside a CUDA graph's capture (it makes the device's status word); after it all calls can be captured
+once validation is off, with lengths and tables that change in place between replays.
+
 As in `packed_varlen_attn` all arithmetic happens in libvafa_b200.so.  With validation on (`set_validate_cu_seqlens`,
 the default) lengths, page ids and positions are checked on the host, which waits for the device; a serving loop
 switches it off.  Unchecked, an index that leaves its array is not followed on the device either: nothing outside the tensors is read or
