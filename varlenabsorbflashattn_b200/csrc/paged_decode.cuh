@@ -58,7 +58,9 @@ struct Config {
   static constexpr int kPBytes = kFp32 ? RG * KW * (KPW + 2) * ROWS_G * 4 : 0;
   static constexpr int kBudget = 227 * 1024;
   static constexpr int kMaxStages = 6;
-  static constexpr int bytes_of(int s) { return s * kStageBytes + kQBytes + kMlBytes + kPBytes + (s + 2) * (16 + BK * 16) + 256; }
+  // Places of keys are held for two blocks, those that are looked up before the loop in the stage that the loop fills first.
+  static constexpr int row_slots(int s) { return (s - 1) * BK * 16 <= kStageBytes ? 2 : s + 1; }
+  static constexpr int bytes_of(int s) { return s * kStageBytes + kQBytes + kMlBytes + kPBytes + row_slots(s) * BK * 16 + (s + 2) * 16 + 256; }
   static constexpr int fit(int ctas) {
     int s = kMaxStages;
     while (s > 1 && (bytes_of(s) + 1024) * ctas > kBudget + 1024) --s;
@@ -176,7 +178,8 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
   float2* const join_ml = reinterpret_cast<float2*>(at); at += C::kMlBytes;
   float* const p_all = reinterpret_cast<float*>(at);   at += C::kPBytes;
   at = smem + (((at - smem) + 15) & ~15);
-  longlong2* const row_at = reinterpret_cast<longlong2*>(at); at += C::kInfo * BK * 16;
+  constexpr int kRowSlots = C::row_slots(S);
+  longlong2* const row_at = reinterpret_cast<longlong2*>(at); at += kRowSlots * BK * 16;
   Block* const info = reinterpret_cast<Block*>(at);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -224,10 +227,13 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
       }
     }
   };
+  auto rows_of = [&](int i) { return row_at + i % kRowSlots * BK; };
+  auto first_rows_of = [&](int i) {  // before the loop
+    return kRowSlots == 2 && i < S - 1 ? reinterpret_cast<longlong2*>(stages + (S - 1) * C::kStageBytes) + i * BK : rows_of(i);
+  };
   // a key's place in bytes from the head's first element; 0 for what lies behind the sequence, -1 for a page that is not there
-  auto land = [&](const Lookup& x, int i) {
-    const int slot = i % C::kInfo;
-    if (tid == 0) info[slot] = x.b;
+  auto land = [&](const Lookup& x, int i, longlong2* rows) {
+    if (tid == 0) info[i % C::kInfo] = x.b;
     longlong2 r = make_longlong2(0, 0);
     if (x.b.seq < p.n_seq && x.b.kb * BK + tid < x.b.len) {
       if (x.page >= 0 && x.page < p.num_pages) {
@@ -238,12 +244,12 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
         report_error(p.status, kBadCacheIndex, kSiteDecode, x.b.seq);
       }
     }
-    row_at[slot * BK + tid] = r;
+    rows[tid] = r;
   };
   // copies block i (of this CTA) into its stage
-  auto issue = [&](int i) {
+  auto issue = [&](int i, const longlong2* places) {
     const Block b = info[i % C::kInfo];
-    const longlong2* const rows = row_at + (i % C::kInfo) * BK + tid / C::CH;
+    const longlong2* const rows = places + tid / C::CH;
     const int h = b.hr & 0xffff;
     unsigned char* const st = stages + (i % S) * C::kStageBytes;
     const char* const kh = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + h * p.k_head) + tid % C::CH * 16;
@@ -290,7 +296,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
       walk();
     }
 #pragma unroll
-    for (int i = 0; i < S; ++i) land(x[i], i);
+    for (int i = 0; i < S; ++i) land(x[i], i, first_rows_of(i));
   }
   Lookup next;
   if (looks_up) {
@@ -300,7 +306,7 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < S - 1; ++i) {
-    if (i < n_iter) issue(i);
+    if (i < n_iter) issue(i, first_rows_of(i));
     copy_commit();
   }
 
@@ -310,10 +316,10 @@ __global__ void __launch_bounds__(C::THREADS, C::CTAS) decode_kernel(const Decod
   for (int i = 0; i < n_iter; ++i) {
     copy_wait<S - 2>();
     __syncthreads();
-    if (i + S - 1 < n_iter) issue(i + S - 1);
+    if (i + S - 1 < n_iter) issue(i + S - 1, rows_of(i + S - 1));
     copy_commit();
     if (looks_up) {
-      land(next, i + S);
+      land(next, i + S, rows_of(i + S));
       start(next);
       walk();
     }
@@ -536,11 +542,11 @@ Plan plan_of(int R) { return Plan{C::ROWS, (R + C::ROWS - 1) / C::ROWS, C::CTAS,
 // The tile of a shape, by the rows of its units and the head dim.  What decides is how many warps there are to hide latencies, then how
 // often an SM reads a block from shared memory.  64 caches of 4k to 8k keys with 8 K/V heads of 128, us:
 //   up to 8 rows     narrow; 1 | 2 | 3 CTAs an SM (128 caches of 8k to 32k keys) 2782 | 1585 | 1427
-//   up to 16         wide, 4 warps on a block, 2 CTAs: 275; with one 442; two warps on a block 351; narrow with two column tiles 292
-//   up to 32         wide, 2 row groups of 2 warps, 2 CTAs: 361; one CTA 592; 2 groups of 4 warps 441; one warp a group 532
-//   up to 64         wide, 4 row groups of 1 warp, 2 CTAs: 534; of 2 warps, one CTA 636; of 4 warps 1165
+//   up to 16         wide, 4 warps on a block, 3 CTAs: 256; two 264, one 442; two warps on a block 351; narrow with two column tiles 292
+//   up to 32         wide, 2 row groups of 2 warps, 2 CTAs: 333; (of the first version) 361; one CTA 592; 4 warps a group 441, one 532
+//   up to 64         wide, 4 row groups of 1 warp, 2 CTAs: 515; (of the first version) 534; of 2 warps, one CTA 636; of 4 warps 1165
 //   heads of 256     O takes twice the registers: narrow with two row groups to 16 rows, 284 (wide 376), wide beyond
-//   fp32             4 rows a warp where units have no more, 3 CTAs: 523; 8 rows 877 (two groups of 4: 851, but no gain with more rows)
+//   fp32             4 rows a warp where units have no more, 3 CTAs: 507; 8 rows 877 (two groups of 4: 851, but no gain with more rows)
 template <typename T, int D>
 Plan plan_for(int R) {
   if constexpr (sizeof(T) == 4) {
