@@ -169,6 +169,7 @@ class _Plan:
                 _lib.check_status(self.device)
 
 
+_PACKED = torch.contiguous_format
 _plans: dict = {}
 _MOST_PLANS = 4096
 
@@ -208,14 +209,13 @@ def _rotary_plan(q, k, cos, positions, cu, interleaved: bool, inverse: bool) -> 
     qs, ks = ((0, 0) if x is None else x.stride()[:2] for x in (q, k))
     a = _lib.RotaryArgs(*[None] * 8, *qs, *ks, 0 if cu is None else cu.numel() - 1, T, H, H_kv, D, 2 * cos.shape[1], cos.shape[0],
                         _lib.DTYPE_CODE[ref.dtype], interleaved, inverse)
-    return _Plan(a, ref.device, "vafa_rotary", out=((T, H, D), (T, H_kv, D)))
+    return _Plan(a, ref.device, "vafa_rotary", out=T)
 
 
 def _rotate(plan: _Plan, q, k, cos, sin, positions, cu):
-    shapes = plan.out
-    qo = None if q is None else q.new_empty(shapes[0])
-    ko = None if k is None else k.new_empty(shapes[1])
-    if shapes[0][0] == 0:
+    qo = None if q is None else torch.empty_like(q, memory_format=_PACKED)
+    ko = None if k is None else torch.empty_like(k, memory_format=_PACKED)
+    if plan.out == 0:
         return qo, ko
     a = plan.args()
     if q is not None:
@@ -431,15 +431,15 @@ def paged_kv_append(
             *[None] * 11, *((0, 0) if q is None else q.stride()[:2]), *k.stride()[:2], *v.stride()[:2], *k_cache.stride()[:3],
             *v_cache.stride()[:3], page_table.stride(0), n_seq, T, 0 if q is None else q.shape[1], H_kv, D, R, rows, num_pages, page_size,
             page_table.shape[1], _lib.DTYPE_CODE[k.dtype], bool(interleaved))
-        plan = _Plan(a, dev, "vafa_paged_append", out=(T, n_seq, None if q is None else (T, q.shape[1], D)))
+        plan = _Plan(a, dev, "vafa_paged_append", out=(T, n_seq))
         if key[1:11] == tuple(map(_layout, (k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens, q, cos, sin))):
             _keep(key, plan)
     if torch.is_grad_enabled():
         _no_gradient("paged_kv_append", k, v, q, k_cache, v_cache, cos, sin)
     kc, vc = k_cache.data_ptr(), v_cache.data_ptr()
     _need(kc != vc, lambda: "k_cache and v_cache are the same memory")
-    T, n_seq, shape = plan.out
-    qo = None if q is None else q.new_empty(shape)
+    T, n_seq = plan.out
+    qo = None if q is None else torch.empty_like(q, memory_format=_PACKED)
     if T > 0 and n_seq > 0:
         if _varlen._validate:
             _check_append(*(None if x is None else _host(x) for x in given), T, k_cache.shape[0], k_cache.shape[1],
@@ -504,7 +504,7 @@ def _decode(q, k_cache, v_cache, page_table, cache_seqlens, scale, with_lse):
         raise ValueError("k_cache, v_cache: base and strides must be multiples of 16 bytes")
     if qp & 15:
         return _decode(q.clone(), k_cache, v_cache, *reversed(given), scale, with_lse)
-    o = q.new_empty(q.shape)
+    o = torch.empty_like(q, memory_format=_PACKED)
     lse = torch.empty(plan.out[0], dtype=torch.float32, device=plan.device) if with_lse else None
     if plan.out[1] == 0:
         return o, lse
