@@ -111,6 +111,23 @@ def test_integer_arguments():
             paged._ints(bad, dev, "x")
 
 
+def test_sizes_beyond_32_bits():
+    # 2^32 + 1 rows would arrive in the library as one
+    many = 2**32 + 1
+    for x in (torch.zeros(1, 1, 64).expand(many, 1, 64), torch.zeros(1, 1, 64).expand(1, many, 64)):
+        with pytest.raises(ValueError, match="int32 range"):
+            paged._rows(x, "q")
+        with pytest.raises(ValueError, match="int32 range"):
+            vb.paged_decode_attn(x, x, x, page_table=torch.zeros(1, 1), cache_seqlens=torch.zeros(1))
+    with pytest.raises(ValueError, match="int32 range"):
+        paged._ints(torch.zeros(1, dtype=torch.int64).expand(many), torch.device("cpu"), "cache_seqlens")
+    table, lens = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for cache in (torch.zeros(1, 16, 1, 64).expand(many, 16, 1, 64), torch.zeros(1, 16, 1, 64).expand(1, 16, many, 64)):
+        with pytest.raises(ValueError, match="int32 range"):
+            paged._check_cache(cache, cache, table, lens, torch.zeros(1, 1, 64))
+    assert paged._counts(torch.zeros(0), "q").numel() == 0 and paged._counts(torch.zeros(()), "q").dim() == 0
+
+
 def test_check_pages():
     table = torch.tensor([[0, 1, 99], [2, -7, 3]])
     paged._check_pages(torch.tensor([8, 4]), table, 4, 4)  # what lies behind the length is nobody's

@@ -37,7 +37,6 @@ struct DecodeParams {
   int32_t* status;
 };
 
-// NT x 8 rows a warp, RG groups of KW warps that share the keys, at most MOST CTAs an SM
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 16 bytes to shared memory; zeros where there is nothing to read.
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {

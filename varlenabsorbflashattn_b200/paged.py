@@ -48,8 +48,16 @@ def _need(ok: bool, message) -> None:
 # ------------------------------------------------------------------------------------------------
 # arguments
 # ------------------------------------------------------------------------------------------------
+def _counts(x: torch.Tensor, name: str) -> torch.Tensor:
+    """The library counts in 32 bits: a size beyond them (an expanded tensor has it for nothing) must not arrive as a smaller one."""
+    if max(x.shape, default=0) > 2**31 - 1:
+        raise ValueError(f"{name}: shape {tuple(x.shape)} exceeds int32 range")
+    return x
+
+
 def _rows(x: torch.Tensor, name: str) -> Tuple[torch.Tensor, bool]:
     """[T, H, D] of a packed tensor, at its own strides as long as the last dim is contiguous."""
+    _counts(x, name)
     was4 = x.dim() == 4
     if was4:
         if x.shape[0] != 1:
@@ -75,6 +83,7 @@ def _ints(t: torch.Tensor, device: torch.device, name: str, dims: int = 1) -> to
     """int32 on the device, the last dim contiguous."""
     if t.dim() != dims:
         raise ValueError(f"{name}: must be {dims}-D, got shape {tuple(t.shape)}")
+    _counts(t, name)
     if t.dtype is not torch.int32 or t.device != device:
         if t.is_floating_point() or t.dtype == torch.bool:
             raise ValueError(f"{name}: must hold integers, got {t.dtype}")
@@ -87,6 +96,7 @@ def _check_angles(cos: torch.Tensor, sin: torch.Tensor, ref: torch.Tensor) -> in
     _need(cos.dtype == sin.dtype == torch.float32, lambda: f"cos/sin must be fp32, got {cos.dtype} and {sin.dtype}")
     _need(cos.device == ref.device and sin.device == ref.device, lambda: "cos/sin must be on the device of q and k")
     _need(cos.is_contiguous() and sin.is_contiguous(), lambda: "cos/sin must be contiguous")
+    _counts(cos, "cos/sin")
     _need(2 <= 2 * cos.shape[1] <= ref.shape[-1], lambda: f"rotary_dim {2 * cos.shape[1]} must be 2 to head_dim {ref.shape[-1]}")
     return 2 * cos.shape[1]
 
@@ -109,7 +119,7 @@ def _host(t: torch.Tensor) -> torch.Tensor:
 def _check_cache(k_cache, v_cache, page_table, cache_seqlens, ref) -> None:
     for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
         _need(c.dim() == 4, lambda: f"{name}: expected [num_pages, page_size, H_kv, D], got shape {tuple(c.shape)}")
-        _like(c, ref, name)
+        _like(_counts(c, name), ref, name)
         _need(c.stride(3) == 1, lambda: f"{name}: the last dim must be contiguous")
     _need(k_cache.shape == v_cache.shape, lambda: f"v_cache shape {tuple(v_cache.shape)}, k_cache {tuple(k_cache.shape)}")
     _need(k_cache.shape[3] == ref.shape[-1], lambda: f"caches have head_dim {k_cache.shape[3]}, the new tokens {ref.shape[-1]}")
@@ -302,7 +312,6 @@ def packed_rotary(
             _like(k, q, "k")
             _need(k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2], lambda: f"K shape mismatch: {tuple(k.shape)} vs q {tuple(q.shape)}")
         _check_angles(cos, sin, q)
-        _lib.check_rows(q.shape[0], cos.shape[0])
         if (cu_seqlens is not None) + (seqinfo is not None) + (positions is not None) != 1:
             raise ValueError("must provide one of cu_seqlens, seqinfo and positions")
         if positions is None:
@@ -409,7 +418,6 @@ def paged_kv_append(
         for c, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
             _need(all(st > 0 or n == 1 for st, n in zip(c.stride(), c.shape)), lambda: f"{name}: an expanded tensor cannot be written to")
         n_seq = cache_seqlens.shape[0]
-        _lib.check_rows(T, n_seq)
         if cu_seqlens is not None:
             cu_seqlens = _ints(cu_seqlens, dev, "cu_seqlens")
             _need(cu_seqlens.shape[0] == n_seq + 1, lambda: f"cu_seqlens has {cu_seqlens.shape[0] - 1} sequences, cache_seqlens {n_seq}")
@@ -472,7 +480,7 @@ def _decode(q, k_cache, v_cache, page_table, cache_seqlens, scale, with_lse):
     if plan is None:
         if q.dim() not in (3, 4):
             raise ValueError(f"q: expected [n_seq,H,D] or [n_seq,T,H,D], got {q.dim()}-D")
-        _check_heads(q, "q")
+        _check_heads(_counts(q, "q"), "q")
         dev = q.device
         cache_seqlens = _ints(cache_seqlens, dev, "cache_seqlens")
         page_table = _ints(page_table, dev, "page_table", 2)
