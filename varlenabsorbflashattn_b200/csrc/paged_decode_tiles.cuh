@@ -11,6 +11,7 @@
 //               the head dim over the lanes for P V.
 // 16-bit P is split into two pieces (hi + lo) for the second product: one piece would put an error of the size of the output's own
 // rounding on top of it (2.4e-3 instead of 1.7e-3 of bf16 outputs); the second costs a product per V fragment and no time that shows.
+// fp16 P is held larger than it is, for its short range (kLift).
 // Keys that some rows see and others do not (the new tokens themselves) are summed apart where V is not finite: 0 times a
 // NaN would reach the rows that do not see it.
 #pragma once
@@ -127,6 +128,22 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t&
   lo = pack2_out<T>(a - to_float(h[0]), b - to_float(h[1]));
 }
 
+// fp16 has no value below 2^-24, and none with all its bits below 2^-14: weights far below the running maximum would lose bits, or
+// be lost, in the second product although l has counted them (a first key 17 nats above 131 000 others that hold all of the
+// values: 0.0078 for 0.0054; 17.4 nats: 0).  So P, and O with it, are held 2^15 times as large there, which no weight overflows; and where
+// a row's largest weight among the warp's keys of a block is below 2^-8, they are lifted by that as well, O brought to the same scale
+// for the block's products and back.  Powers of two: nothing is rounded.  O stays below 2^122: 2^31 keys, values of 2^16, 2^15, 2^60.
+// What a weight can lose is then 2^-40 of the largest one that the warp has at once, with the keys beside it.
+// (Without | with, us: 64 caches of 1k to 16k keys, 32 query and 8 K/V heads of 128 370 | 370, also where every block is lifted;
+// 64 of 4k to 8k, four tokens of 4 grouped heads 256.5 | 257.9, of 8 333 | 336, seven of 8 527 | 536.)
+template <typename T> constexpr int kLift = std::is_same<T, __half>::value ? 15 : 0;
+__device__ __forceinline__ float pow2(int k) { return __int_as_float((127 + k) << 23); }
+// `top`: the largest score of the keys, `now`: the running maximum.  (Not where there is no score, nor where every weight is zero.)
+__device__ __forceinline__ int lift_of(float top, float now) {
+  const float gap = now - top;
+  return gap > 8.f && gap < 150.f ? (int)fminf(gap, 60.f) : 0;
+}
+
 template <typename C>
 struct NarrowTile {
   using T = typename C::T;
@@ -194,7 +211,8 @@ struct NarrowTile {
         if (b.masked && (j0 + 16 * t + (x >> 1) * 8 >= limit[x & 1])) s[t][x] = -INFINITY;
       }
     float alpha[2];
-    bool moved = false;
+    int lift[2];
+    bool moved = false, far = false;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       float top = fmaxf(s[0][x], s[0][x + 2]);
@@ -216,8 +234,18 @@ struct NarrowTile {
       }
       l[x] = l[x] * alpha[x] + sum;
       m[x] = now;
+      if constexpr (kLift<T> != 0) {
+        lift[x] = lift_of(top, now);
+        far |= lift[x] != 0;
+        alpha[x] *= pow2(lift[x]);
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          s[t][x] *= pow2(kLift<T> + lift[x]);
+          s[t][x + 2] *= pow2(kLift<T> + lift[x]);
+        }
+      }
     }
-    if (__any_sync(0xffffffffu, moved)) {
+    if (__any_sync(0xffffffffu, moved || far)) {
 #pragma unroll
       for (int d = 0; d < D / 16; ++d)
 #pragma unroll
@@ -286,6 +314,14 @@ struct NarrowTile {
         }
       }
     }
+    if constexpr (kLift<T> != 0) {
+      if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[d][x] *= pow2(-lift[x & 1]);
+      }
+    }
   }
 
   // the warp's (m, l) of its row group's rows
@@ -303,7 +339,7 @@ struct NarrowTile {
 #pragma unroll
     for (int d = 0; d < D / 16; ++d)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) out[(2 * (lane & 3) + (x & 1)) * C::MP + d * 16 + (lane >> 2) + (x >> 1) * 8] = o[d][x];
+      for (int x = 0; x < 4; ++x) out[(2 * (lane & 3) + (x & 1)) * C::MP + d * 16 + (lane >> 2) + (x >> 1) * 8] = o[d][x] * pow2(-kLift<T>);
   }
 };
 
@@ -394,7 +430,8 @@ struct WideTile {
         if (b.masked && (j0 + 8 * j + (x & 1) >= limit[x >> 1])) s[j][x] = -INFINITY;
       }
     float alpha[2];
-    bool moved = false;
+    int lift[2];
+    bool moved = false, far = false;
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       float top = fmaxf(s[0][2 * x], s[0][2 * x + 1]);
@@ -416,8 +453,17 @@ struct WideTile {
         }
       l[x] = l[x] * alpha[x] + sum;
       m[x] = now;
+      if constexpr (kLift<T> != 0) {
+        lift[x] = lift_of(top, now);
+        far |= lift[x] != 0;
+        alpha[x] *= pow2(lift[x]);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) s[j][2 * x + e] *= pow2(kLift<T> + lift[x]);
+      }
     }
-    if (__any_sync(0xffffffffu, moved)) {
+    if (__any_sync(0xffffffffu, moved || far)) {
 #pragma unroll
       for (int n = 0; n < D / 8; ++n)
 #pragma unroll
@@ -490,6 +536,14 @@ struct WideTile {
         }
       }
     }
+    if constexpr (kLift<T> != 0) {
+      if (__any_sync(0xffffffffu, far)) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[n][x] *= pow2(-lift[x >> 1]);
+      }
+    }
   }
 
   __device__ __forceinline__ void stats(float2* out) {
@@ -502,9 +556,10 @@ struct WideTile {
   }
   __device__ __forceinline__ void rows(float* out, int half) const {
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-      *reinterpret_cast<float2*>(out + (lane >> 2) * C::MP + 8 * n + 2 * (lane & 3)) =
-          half ? make_float2(o[n][2], o[n][3]) : make_float2(o[n][0], o[n][1]);
+    for (int n = 0; n < D / 8; ++n) {
+      const float a = half ? o[n][2] : o[n][0], b = half ? o[n][3] : o[n][1];
+      *reinterpret_cast<float2*>(out + (lane >> 2) * C::MP + 8 * n + 2 * (lane & 3)) = make_float2(a * pow2(-kLift<T>), b * pow2(-kLift<T>));
+    }
   }
 };
 
