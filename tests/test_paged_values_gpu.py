@@ -1,5 +1,5 @@
 """Paged decode where the values are what is hard: fp16 weights far below the largest one, held to a bound without a floor that grows with
-the number of keys."""
+the number of keys, and infinite values that a row sees."""
 import pytest
 import torch
 
@@ -72,5 +72,36 @@ def test_fp16_scores_of_large_spread(D, H, H_kv, T):
     o, lse = vb.paged_decode_attn_with_lse(q, kc, vc, page_table=table, cache_seqlens=_ints(lens), scale=scale)
     # the steps' largest weights add up to no more than all weights, 1
     ro, rl, eo, el = _decode_fp16(q, kc, vc, table, lens, scale, 64 * 2.0 ** -32 * vc.abs().max().item())
+    assert_within(lse, rl, el, "lse")
+    assert_within(o, ro, eo, "o")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D,H,H_kv,T", TILES)
+def test_infinite_values_that_a_row_sees(dtype, D, H, H_kv, T):
+    """An infinite value is an infinite result of the rows that see it, whatever its weight is, and two of opposite signs are NaN; the other
+    dims, and the rows that do not see it, are as the formula has them."""
+    gen, lens, inf = _gen(D), [1, 300, 20, 90, 5000, T], float("inf")
+    kc, vc, table = paged_cache(lens, H_kv, D, 16, dtype, gen)
+    q = _randn(gen, len(lens), T, H, D, dtype=dtype)
+
+    def put(seq, key, dim, value):
+        vc[table[seq, key // 16].long(), key % 16, :, dim] = value
+
+    put(0, 0, 0, inf)                                   # the only weight, 1
+    for key, dim, value in ((7, 3, inf), (250, 3, inf), (100, 5, -inf), (31, 6, inf), (40, 6, -inf), (299, 8, inf), (0, 9, -inf)):
+        put(1, key, dim, value)
+    for dim in range(D):
+        put(2, 19, dim, -inf)                           # of several tokens only the last one sees it
+    kc[table[3, :6].long()] = 0                         # a weight of 2^-29 beside the first key's
+    q[3] = 0
+    kc[table[3, 0].long(), 0, :, 0], q[3, ..., 0], vc[table[3, 0].long(), 0] = 20 * D ** 0.5 / 4, 4, 0
+    put(3, 50, 1, inf)
+    for key in range(4321, 4400):
+        put(4, key, D - 1, inf)
+    put(5, T - 1, 2, inf)
+    ro, rl, eo, el = decode(q, kc, vc, table, lens)
+    assert torch.isinf(ro).any() and ro.isnan().any()
+    o, lse = vb.paged_decode_attn_with_lse(q, kc, vc, page_table=table, cache_seqlens=_ints(lens))
     assert_within(lse, rl, el, "lse")
     assert_within(o, ro, eo, "o")
