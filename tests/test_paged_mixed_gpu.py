@@ -1,0 +1,64 @@
+"""Rotation, paged append and paged decode on the GPU: arguments of other types and kinds than the usual ones."""
+import pytest
+import torch
+
+import varlenabsorbflashattn_b200 as vb
+from varlenabsorbflashattn_b200 import _lib
+from paged_ref import paged_cache
+
+pytestmark = pytest.mark.gpu
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture
+def unchecked():
+    vb.set_validate_cu_seqlens(False)
+    yield
+    vb.set_validate_cu_seqlens(True)
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(gen, *shape, dtype=F32):
+    return torch.randn(shape, generator=gen, device="cuda").to(dtype)
+
+
+def _cu(lens):
+    return torch.tensor([0] + list(lens)).cumsum(0).to(torch.int32).cuda()
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _status():
+    st = _lib.status_word(torch.device("cuda", 0))
+    got = st.tolist()
+    st.zero_()
+    return got[:2]
+
+
+def test_unchecked_indices_beyond_32_bits(unchecked):
+    """2^32 + 3 is not page 3, nor 2^32 + 8 a length of 8: out of range like any other, reported, nothing written."""
+    gen, wide = _gen(1), 2**32
+    kc, vc, table = paged_cache([8, 8, 8], 2, 64, 4, BF16, gen, fill=0.0)
+    q, k, v = (_randn(gen, 3, 2, 64, dtype=BF16) for _ in range(3))
+    cos, sin = vb.rotary_table(8, 64, device="cuda")
+    lens = torch.tensor([8, 8, 8], device="cuda")
+    before = kc.clone(), vc.clone()
+    call = lambda lens, table: vb.paged_kv_append(k, v, kc, vc, page_table=table, cache_seqlens=lens, q=q, cos=cos, sin=sin)  # noqa: E731
+    _status()
+    assert call(lens, table.long() + wide).isnan().all() and _status() == [4, 911]
+    assert call(lens, table.long() - wide).isnan().all() and _status() == [4, 911]
+    assert call(lens + wide, table).isnan().all() and _status() == [4, 911]
+    assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+    got, _ = vb.packed_rotary(q, None, cos, sin, positions=torch.tensor([1, wide, 2 - wide]))
+    assert got[1:].isnan().all() and not got[0].isnan().any() and _status() == [4, 910]
+
+    want = vb.paged_decode_attn(q, kc, vc, page_table=table, cache_seqlens=lens)
+    for lens_, table_ in ((lens + torch.tensor([0, wide, 0], device="cuda"), table), (lens, table.long() + torch.tensor([[0], [wide], [0]], device="cuda"))):
+        assert _status() == [0, 0]
+        got = vb.paged_decode_attn(q, kc, vc, page_table=table_, cache_seqlens=lens_)
+        assert _status() == [4, 912] and torch.equal(got[[0, 2]], want[[0, 2]])

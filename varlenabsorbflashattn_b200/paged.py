@@ -79,14 +79,19 @@ def _like(x: torch.Tensor, ref: torch.Tensor, name: str) -> None:
     _need(x.dtype == ref.dtype, lambda: f"{name}: dtype {x.dtype}, the others have {ref.dtype}")
 
 
+_WIDE = (torch.int64, torch.uint64, torch.uint32)
+
+
 def _ints(t: torch.Tensor, device: torch.device, name: str, dims: int = 1) -> torch.Tensor:
-    """int32 on the device, the last dim contiguous."""
+    """int32 on the device, the last dim contiguous; values beyond 32 bits as the nearest ones, which the kernels refuse as they do those."""
     if t.dim() != dims:
         raise ValueError(f"{name}: must be {dims}-D, got shape {tuple(t.shape)}")
     _counts(t, name)
     if t.dtype is not torch.int32 or t.device != device:
         if t.is_floating_point() or t.dtype == torch.bool:
             raise ValueError(f"{name}: must hold integers, got {t.dtype}")
+        if t.dtype in _WIDE:  # what 32 bits do not hold must not arrive as something that they do
+            t = t.to(torch.int64).clamp(-2**31, 2**31 - 1)
         t = t.to(device=device, dtype=torch.int32)
     return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
 
