@@ -1,7 +1,9 @@
 """Rotation, paged append and paged decode without a GPU: arguments of other types and kinds than the usual ones."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
+import varlenabsorbflashattn_b200 as vb
 from varlenabsorbflashattn_b200 import paged
 
 
@@ -18,3 +20,24 @@ def test_integers_of_32_bits_and_less_stay_as_they_are():
     assert paged._ints(x, x.device, "x") is x
     for dtype in (torch.int8, torch.int16):
         assert paged._ints(x.to(dtype), x.device, "x").tolist() == [5, -3]
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_is_refused_by_every_call(grad_mode):
+    """No result without its tangent: neither requires_grad nor grad mode has a part in it."""
+    x, c = torch.zeros(3, 2, 16), torch.zeros(4, 8)
+    cache, table, lens = torch.zeros(2, 4, 2, 16), torch.zeros(3, 1, dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    where = dict(page_table=table, cache_seqlens=lens)
+    cu = torch.tensor([0, 3])
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: vb.packed_rotary(dual(x), None, c, c, cu_seqlens=cu), lambda: vb.packed_rotary(x, dual(x), c, c, cu_seqlens=cu),
+                     lambda: vb.packed_rotary(x, x, c, dual(c), cu_seqlens=cu), lambda: vb.paged_kv_append(dual(x), x, cache, cache, **where),
+                     lambda: vb.paged_kv_append(x, dual(x), cache, cache, **where),
+                     lambda: vb.paged_kv_append(x, x, cache, cache, q=dual(x), cos=c, sin=c, **where),
+                     lambda: vb.paged_decode_attn(dual(x), cache, cache, **where), lambda: vb.paged_decode_attn(x, cache, dual(cache), **where),
+                     lambda: vb.paged_decode_attn_with_lse(x, dual(cache), cache, **where)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with pytest.raises(AssertionError, match="CUDA"):  # a call without a tangent goes on to the other checks
+            vb.packed_rotary(x, None, c, c, cu_seqlens=cu)

@@ -1,6 +1,7 @@
 """Rotation, paged append and paged decode on the GPU: arguments of other types and kinds than the usual ones."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import varlenabsorbflashattn_b200 as vb
 from varlenabsorbflashattn_b200 import _lib
@@ -62,3 +63,29 @@ def test_unchecked_indices_beyond_32_bits(unchecked):
         assert _status() == [0, 0]
         got = vb.paged_decode_attn(q, kc, vc, page_table=table_, cache_seqlens=lens_)
         assert _status() == [4, 912] and torch.equal(got[[0, 2]], want[[0, 2]])
+
+
+def test_forward_mode_is_refused():
+    gen = _gen(2)
+    kc, vc, table = paged_cache([8, 8], 2, 64, 4, F32, gen, fill=0.0)
+    before = kc.clone(), vc.clone()
+    q, t = _randn(gen, 2, 2, 64), _randn(gen, 2, 2, 64)
+    cos, sin = vb.rotary_table(8, 64, device="cuda")
+    where = dict(page_table=table, cache_seqlens=_ints([8, 8]))
+    for _ in range(2):  # a layout that has been called before, and one that has not
+        with forward_ad.dual_level():
+            x = forward_ad.make_dual(q, t)
+            for call in (lambda: vb.packed_rotary(x, None, cos, sin, cu_seqlens=_cu([2])), lambda: vb.paged_kv_append(q, x, kc, vc, **where),
+                         lambda: vb.paged_decode_attn(x, kc, vc, **where)):
+                with pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+        vb.packed_rotary(q, None, cos, sin, cu_seqlens=_cu([2]))
+        vb.paged_kv_append(q, q, kc, vc, **where)
+        vb.paged_decode_attn(q, kc, vc, **where)
+        before = kc.clone(), vc.clone()
+    rotated = lambda x: vb.packed_rotary(x, None, cos, sin, cu_seqlens=_cu([2]))[0]  # noqa: E731
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(rotated, (q,), (t,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(rotated)(q[None])

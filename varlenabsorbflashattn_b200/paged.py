@@ -31,6 +31,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from . import varlen as _varlen
@@ -111,6 +112,14 @@ def _no_gradient(what: str, *tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach its inputs")
+
+
+def _no_tangent(what: str, *tensors) -> None:
+    """Forward mode asks neither for requires_grad nor for grad mode: a tangent would be dropped in silence."""
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{what} has no forward-mode derivative")
 
 
 def _host(t: torch.Tensor) -> torch.Tensor:
@@ -289,7 +298,7 @@ def packed_rotary(
     positions: Optional[torch.Tensor] = None,
     interleaved: bool = False,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
-    """Rotate packed queries and keys by their positions, in one launch; differentiable in q and k.
+    """Rotate packed queries and keys by their positions, in one launch; differentiable in q and k (in reverse mode).
 
     q: [T, H, D] or [1, T, H, D], k: [T, H_kv, D] or [1, T, H_kv, D], or None (fp32, bf16 or fp16; D as in
     `packed_varlen_attn`).  Tokens and heads may be strided, as in views of one projection's output.
@@ -303,6 +312,7 @@ def packed_rotary(
     A step with its gradients can be captured into a CUDA graph once validation is off; as with every operator, torch wants no
     eager autograd graph of the same leaves to be alive meanwhile (its AccumulateGrad nodes belong to the eager stream).
     """
+    _no_tangent("packed_rotary", q, k, cos, sin)
     if seqinfo is not None and cu_seqlens is None and positions is None:
         cu_seqlens, seqinfo = _lengths_to_cu(seqinfo), None
     key = ("packed_rotary", _layout(q), _layout(k), _layout(cos), _layout(sin), _layout(cu_seqlens), _layout(positions), seqinfo is None, interleaved)
@@ -400,6 +410,7 @@ def paged_kv_append(
     Sequences may share pages that are only read (a common prefix); what is written must be theirs alone.
     Returns the rotated q (contiguous; zeros for padding), or None without q.  Has no gradient.
     """
+    _no_tangent("paged_kv_append", k, v, q, k_cache, v_cache, cos, sin)
     if seqinfo is not None and cu_seqlens is None:
         cu_seqlens = _lengths_to_cu(seqinfo)
     tensors = (k, v, k_cache, v_cache, page_table, cache_seqlens, cu_seqlens, q, cos, sin)
@@ -478,6 +489,7 @@ def paged_kv_append(
 # attention
 # ------------------------------------------------------------------------------------------------
 def _decode(q, k_cache, v_cache, page_table, cache_seqlens, scale, with_lse):
+    _no_tangent("paged_decode_attn", q, k_cache, v_cache)
     tensors = (q, k_cache, v_cache, page_table, cache_seqlens)
     key = ("paged_decode_attn", *map(_layout, tensors), scale)
     plan = _plans.get(key)
