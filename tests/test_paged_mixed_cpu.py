@@ -41,3 +41,20 @@ def test_forward_mode_is_refused_by_every_call(grad_mode):
                 call()
         with pytest.raises(AssertionError, match="CUDA"):  # a call without a tangent goes on to the other checks
             vb.packed_rotary(x, None, c, c, cu_seqlens=cu)
+
+
+@pytest.mark.parametrize("wants_q,wants_k", [(True, False), (False, True), (True, True)])
+def test_only_what_has_a_gradient_comes_back_with_one(monkeypatch, wants_q, wants_k):
+    monkeypatch.setattr(paged, "_rotate", lambda plan, q, k, *rest: tuple(None if x is None else x.clone() for x in (q, k)))
+    monkeypatch.setattr(paged, "_rotary_plan", lambda *a: None)
+    monkeypatch.setattr(paged, "_plans", {})
+    q, k = (torch.randn(3, 2, 16).requires_grad_(wants) for wants in (wants_q, wants_k))
+    c, cu = torch.zeros(4, 8), torch.tensor([0, 3], dtype=torch.int32)
+    a, b = paged._PackedRotary.apply(q, k, c, c, None, cu, None, False, False)
+    assert (a.requires_grad, b.requires_grad) == (wants_q, wants_k)
+    (a.sum() + b.sum()).backward()
+    assert (q.grad is not None, k.grad is not None) == (wants_q, wants_k)
+    x = torch.randn(3, 2, 16, requires_grad=True)  # and without the other input at all
+    a, b = paged._PackedRotary.apply(x, None, c, c, None, cu, None, False, False)
+    a.sum().backward()
+    assert b is None and torch.equal(x.grad, torch.ones_like(x))

@@ -89,3 +89,18 @@ def test_forward_mode_is_refused():
         torch.func.jvp(rotated, (q,), (t,))
     with pytest.raises(RuntimeError):
         torch.func.vmap(rotated)(q[None])
+
+
+def test_keys_rotated_beside_queries_with_a_gradient_have_none():
+    """With frozen keys the rotated ones go into the cache while queries are trained, and dK is nobody's."""
+    gen = _gen(3)
+    kc, vc, table = paged_cache([8, 8], 2, 64, 4, F32, gen, fill=0.0)
+    q, k = _randn(gen, 2, 4, 64).requires_grad_(), _randn(gen, 2, 2, 64)
+    cos, sin = vb.rotary_table(8, 64, device="cuda")
+    a, b = vb.packed_rotary(q, k, cos, sin, positions=_ints([7, 7]))
+    assert a.requires_grad and not b.requires_grad
+    vb.paged_kv_append(b, k, kc, vc, page_table=table, cache_seqlens=_ints([8, 8]))
+    a, b = vb.packed_rotary(q.detach(), k.requires_grad_(), cos, sin, positions=_ints([7, 7]))
+    assert b.requires_grad and not a.requires_grad
+    g, = torch.autograd.grad(b, k, torch.ones_like(b), create_graph=True)  # the gradient's own graph
+    assert g.shape == k.shape

@@ -263,7 +263,10 @@ class _PackedRotary(torch.autograd.Function):
         ctx.save_for_backward(cos, sin, positions if cu is None else cu)
         ctx.flags = cu is None, interleaved, inverse
         ctx.set_materialize_grads(False)
-        return _rotate(plan, q, k, cos, sin, positions, cu)
+        out = _rotate(plan, q, k, cos, sin, positions, cu)
+        # (what is rotated beside an input with a gradient has none itself)
+        ctx.mark_non_differentiable(*(y for y, needed in zip(out, ctx.needs_input_grad) if y is not None and not needed))
+        return out
 
     @staticmethod
     def backward(ctx, dq, dk):
