@@ -1,10 +1,13 @@
 """Rotation, paged append and paged decode without a GPU: arguments of other types and kinds than the usual ones."""
+import os
+import re
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import varlenabsorbflashattn_b200 as vb
-from varlenabsorbflashattn_b200 import paged
+from varlenabsorbflashattn_b200 import build, paged
 
 
 @pytest.mark.parametrize("dtype", [torch.int64, torch.uint32, torch.uint64])
@@ -58,3 +61,18 @@ def test_only_what_has_a_gradient_comes_back_with_one(monkeypatch, wants_q, want
     a, b = paged._PackedRotary.apply(x, None, c, c, None, cu, None, False, False)
     a.sum().backward()
     assert b is None and torch.equal(x.grad, torch.ones_like(x))
+
+
+def test_warps_whose_lanes_meet_again_give_up_together():
+    """A wait that runs out is each lane's own verdict.  Where lanes shuffle, vote or wait for one another after it, it has to be one for all, or
+    those that stay wait without a limit for those that left.  (Read from the source: no wait is made to run out.)"""
+    with open(os.path.join(build.CSRC, "paged_rotary_rows.cu")) as f:
+        source = re.sub(r"//[^\n]*", "", f.read())
+    kernel = source[source.index("rows_kernel"):source.index("launch_one")]
+    roles = re.split(r"\n  (?:if|\} else if|\} else) ?(?:\(warp [^\n]*\))? ?\{\n", kernel)[1:]
+    assert len(roles) >= 3, "load, store and rotation warps"
+    meets = [r for r in roles if re.search(r"_sync\(|__syncwarp", r.split("\n  }\n")[0])]
+    assert len(meets) >= 2
+    for role in meets:
+        role = role.split("\n  }\n")[0]
+        assert "mbar_wait_warp(" in role and not re.search(r"mbar_wait\(", role), role

@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const Params p, const
       const int run = !turns || !leads ? 0 : leaders ? __ffs(leaders) : w.tokens - token;
       const int rows = mine && token == 0 ? (int)(p.total - t < w.tokens ? p.total - t : w.tokens) : 0;  // of the tile, for its first lane
       for (int i = 0; i < per_batch && batch + (int64_t)i * gridDim.x < w.tiles; ++i, ++sent) {
-        ok = mbar_wait(smem_u32(&ctl.empty[stage]), phase ^ 1, abort_flag);
+        ok = mbar_wait_warp(smem_u32(&ctl.empty[stage]), phase ^ 1, abort_flag);  // one answer: the lanes meet again in the next batch
         if (!ok) break;
         const uint32_t bar = smem_u32(&ctl.full[stage]);
         if (mine && of_batch == i) {
@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, 1) rows_kernel(const Params p, const
     const int behind = w.stages / 2 - 1;
     int sent = 0;
     for (int64_t tile = blockIdx.x; tile < w.tiles; tile += gridDim.x, ++sent) {
-      if (!mbar_wait(smem_u32(&ctl.done[stage]), phase, abort_flag)) break;
+      if (!mbar_wait_warp(smem_u32(&ctl.done[stage]), phase, abort_flag)) break;
       const int64_t t = tile * w.tokens + lane;
       if (lane < w.tokens && t < p.total) {
         const int4 info = ctl.info[stage][lane];
