@@ -7,7 +7,7 @@ import torch
 from torch.autograd import forward_ad
 
 import varlenabsorbflashattn_b200 as vb
-from varlenabsorbflashattn_b200 import build, paged
+from varlenabsorbflashattn_b200 import _lib, build, paged
 
 
 @pytest.mark.parametrize("dtype", [torch.int64, torch.uint32, torch.uint64])
@@ -76,3 +76,11 @@ def test_warps_whose_lanes_meet_again_give_up_together():
     for role in meets:
         role = role.split("\n  }\n")[0]
         assert "mbar_wait_warp(" in role and not re.search(r"mbar_wait\(", role), role
+
+
+def test_status_word_made_under_inference_mode_can_be_cleared(monkeypatch):
+    monkeypatch.setattr(_lib, "_status", {})
+    with torch.inference_mode():
+        word = _lib.status_word(torch.device("cpu", 0))
+    word.zero_()
+    assert not word.is_inference() and _lib.status_word(torch.device("cpu", 0)) is word

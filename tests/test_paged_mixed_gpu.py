@@ -104,3 +104,18 @@ def test_keys_rotated_beside_queries_with_a_gradient_have_none():
     assert b.requires_grad and not a.requires_grad
     g, = torch.autograd.grad(b, k, torch.ones_like(b), create_graph=True)  # the gradient's own graph
     assert g.shape == k.shape
+
+
+def test_errors_of_a_server_under_inference_mode(monkeypatch, unchecked):
+    """The first call of a program may be one of a serving loop: its status word is read and cleared anywhere."""
+    from varlenabsorbflashattn_b200 import paged
+    monkeypatch.setattr(_lib, "_status", {})
+    monkeypatch.setattr(paged, "_plans", {})
+    gen, dev = _gen(4), torch.device("cuda", 0)
+    kc, vc, table = paged_cache([8, 8], 2, 64, 4, BF16, gen, fill=0.0)
+    q = _randn(gen, 2, 2, 64, dtype=BF16)
+    with torch.inference_mode():
+        vb.paged_decode_attn(q, kc, vc, page_table=table + 99, cache_seqlens=_ints([8, 8]))
+    with pytest.raises(RuntimeError, match="outside its array"):
+        _lib.check_status(dev)
+    _lib.check_status(dev)

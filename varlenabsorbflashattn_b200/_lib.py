@@ -174,7 +174,8 @@ def status_word(device: torch.device) -> torch.Tensor:
     key = (device.type, device.index if device.index is not None else torch.cuda.current_device())
     t = _status.get(key)
     if t is None:
-        t = torch.zeros(STATUS_WORDS, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # (made by a first call under inference mode it could not be cleared outside)
+            t = torch.zeros(STATUS_WORDS, dtype=torch.int32, device=device)
         _status[key] = t
     return t
 
