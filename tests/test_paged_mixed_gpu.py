@@ -119,3 +119,18 @@ def test_errors_of_a_server_under_inference_mode(monkeypatch, unchecked):
     with pytest.raises(RuntimeError, match="outside its array"):
         _lib.check_status(dev)
     _lib.check_status(dev)
+
+
+@pytest.mark.parametrize("kept", ["k", "v"])
+def test_autograd_is_told_of_either_cache(kept):
+    """One cache made under inference mode, the other one kept for a gradient."""
+    gen = _gen(5)
+    caches, table = {}, _ints([[0, 1], [2, 3]])
+    with torch.inference_mode():
+        caches["v" if kept == "k" else "k"] = _randn(gen, 4, 4, 2, 64)
+    caches[kept] = _randn(gen, 4, 4, 2, 64)
+    k, w = _randn(gen, 2, 2, 64), torch.ones((), device="cuda", requires_grad=True)
+    y = (w * caches[kept]).sum()
+    vb.paged_kv_append(k, k, caches["k"], caches["v"], page_table=table, cache_seqlens=_ints([8, 8]))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()

@@ -481,8 +481,10 @@ def paged_kv_append(
         if q is not None:
             a.q, a.q_out = q.data_ptr(), qo.data_ptr()
         plan.run(a, "vafa_paged_append")
-        if not k_cache.is_inference():  # autograd is told, as by every operation in place
-            torch.autograd.graph.increment_version((k_cache, v_cache))
+        # autograd is told, as by every operation in place (tensors of inference mode have no version)
+        told = [c for c in (k_cache, v_cache) if not c.is_inference()]
+        if told:
+            torch.autograd.graph.increment_version(told)
     elif qo is not None:
         qo.zero_()
     return qo.unsqueeze(0) if q4 else qo
