@@ -84,3 +84,34 @@ def test_status_word_made_under_inference_mode_can_be_cleared(monkeypatch):
         word = _lib.status_word(torch.device("cpu", 0))
     word.zero_()
     assert not word.is_inference() and _lib.status_word(torch.device("cpu", 0)) is word
+
+
+FAKE = 1 << 20  # an address that no check follows
+
+
+@pytest.fixture(scope="module")
+def lib():
+    build.build()
+    return _lib.load()
+
+
+_ROTARY = dict(q=FAKE, q_out=FAKE, k=FAKE, k_out=FAKE, cos=FAKE, sin=FAKE, cu_seqlens=FAKE, positions=FAKE, n_seg=1, total=4, num_heads=2,
+               num_kv_heads=1, head_dim=64, rotary_dim=64, table_rows=8, dtype=1, status=FAKE)
+_APPEND = dict(q=FAKE, q_out=FAKE, k=FAKE, v=FAKE, k_cache=FAKE, v_cache=FAKE, cos=FAKE, sin=FAKE, rotary_dim=64, table_rows=8, cu_seqlens=FAKE,
+               cache_seqlens=FAKE, page_table=FAKE, n_seq=2, total=2, num_heads=2, num_kv_heads=2, head_dim=64, num_pages=4, page_size=16,
+               max_pages=2, dtype=1, status=FAKE)
+_DECODE = dict(q=FAKE, k_cache=FAKE, v_cache=FAKE, o=FAKE, lse=FAKE, cache_seqlens=FAKE, page_table=FAKE, n_seq=2, q_len=1, num_heads=8, num_kv_heads=2,
+               head_dim=64, num_pages=4, page_size=16, max_pages=8, dtype=1, scale=1.0, sm_count=148, workspace=FAKE, workspace_bytes=1 << 30, status=FAKE)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_addresses_inside_an_element_are_refused(lib, dtype):
+    """What a kernel would read or write across an element's border ends a process on the GPU: refused on the host."""
+    half = 2 if dtype == 0 else 1
+    for entry, struct, good, tensors, words in (
+            (lib.vafa_rotary, _lib.RotaryArgs, _ROTARY, "q k q_out k_out", "positions cu_seqlens status"),
+            (lib.vafa_paged_append, _lib.PagedAppendArgs, _APPEND, "q k v q_out k_cache v_cache", "cu_seqlens cache_seqlens page_table status"),
+            (lib.vafa_paged_decode, _lib.PagedAttnArgs, _DECODE, "", "lse cache_seqlens page_table status")):
+        for name, off in [(n, half) for n in tensors.split()] + [(n, 2) for n in words.split()]:
+            assert entry(struct(**{**good, "dtype": dtype, name: FAKE + off}), None) == -1, name
+            assert "aligned" in _lib.last_error(), (name, _lib.last_error())

@@ -1,6 +1,8 @@
 // C ABI of the rotation, the paged append and the paged decode: argument checks and the choice of a decode tile.
 #include <string.h>
 
+#include <initializer_list>
+
 #include "paged_decode.cuh"
 
 namespace vafa {
@@ -9,6 +11,15 @@ namespace {
 bool dtype_ok(int d) { return d == VAFA_F32 || d == VAFA_BF16 || d == VAFA_F16; }
 bool dim_ok(int d) { return d == 16 || d == 32 || d == 64 || d == 128 || d == 256; }
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Addresses of whole elements, and of whole 32-bit words.
+int check_addresses(int dtype, std::initializer_list<const void*> tensors, std::initializer_list<const void*> words) {
+  for (const void* p : tensors)
+    if (!aligned(p, elem_size(dtype))) return fail(VAFA_ERR_INVALID, "tensors must be aligned to their elements");
+  for (const void* p : words)
+    if (!aligned(p, 4)) return fail(VAFA_ERR_INVALID, "positions, lengths, tables, lse and status must be 4-byte aligned");
+  return 0;
+}
 
 int check_table(const float* cos, const float* sin, int R, int D, int rows) {
   if (!cos || !sin) return fail(VAFA_ERR_INVALID, "null cos/sin");
@@ -132,6 +143,7 @@ int vafa_rotary(const vafa_rotary_args* a, vafa_stream_t stream) {
   if (!a->positions && (!a->cu_seqlens || a->n_seg < 1)) return fail(VAFA_ERR_INVALID, "neither positions nor cu_seqlens");
   if (a->total > 0 && ((a->num_heads > 0 && (!a->q || !a->q_out)) || (a->num_kv_heads > 0 && (!a->k || !a->k_out))))
     return fail(VAFA_ERR_INVALID, "null q/k");
+  if (const int rc = check_addresses(a->dtype, {a->q, a->k, a->q_out, a->k_out}, {a->positions, a->cu_seqlens, a->status})) return rc;
   return rotary_launch(a, (cudaStream_t)stream);
 }
 
@@ -150,6 +162,8 @@ int vafa_paged_append(const vafa_paged_append_args* a, vafa_stream_t stream) {
   if ((rc = check_cache(a->n_seq, a->num_pages, a->page_size, a->max_pages))) return rc;
   if (!a->cu_seqlens && a->total != a->n_seq) return fail(VAFA_ERR_INVALID, "without cu_seqlens total %d must be n_seq %d", a->total, a->n_seq);
   if (a->total > 0 && (!a->k || !a->v || (a->q && !a->q_out))) return fail(VAFA_ERR_INVALID, "null k/v/q_out");
+  if ((rc = check_addresses(a->dtype, {a->q, a->k, a->v, a->q_out, a->k_cache, a->v_cache}, {a->cu_seqlens, a->cache_seqlens, a->page_table, a->status})))
+    return rc;
   return paged_append_launch(a, (cudaStream_t)stream);
 }
 
@@ -168,6 +182,7 @@ int vafa_paged_decode(const vafa_paged_attn_args* a, vafa_stream_t stream) {
                           of(a->num_kv_heads, a->k_cache_head_stride | a->v_cache_head_stride);
   if (!aligned(a->q, 16) || !aligned(a->k_cache, 16) || !aligned(a->v_cache, 16) || !aligned(a->o, 16) || (strides * es) % 16)
     return fail(VAFA_ERR_INVALID, "q, o and the caches need 16-byte aligned bases and strides");
+  if (const int rc = check_addresses(a->dtype, {}, {a->cache_seqlens, a->page_table, a->lse, a->status})) return rc;
   return paged_decode_launch(a, (cudaStream_t)stream);
 }
 
