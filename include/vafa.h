@@ -216,7 +216,7 @@ int vafa_cast_from_f32(const float* src, void* dst, size_t n, int32_t dtype, vaf
  * array and heads may come before slots).  Token j of sequence s lies in slot j % page_size of page
  * page_table[s * table_stride + j / page_size].  Lengths, page ids and positions are read on the device: one that leaves its
  * array is not followed, and code 4 goes to the status word.  Addresses are those of whole elements, whatever the
- * strides (the decode asks for 16 bytes).
+ * strides (the decode asks for 16 bytes); at most 2^30 heads (rotation, append) and sequences (decode).
  * ------------------------------------------------------------------------------------- */
 typedef struct vafa_rotary_args {
   const void* q;        /* [total, H, D], strides below; NULL with num_heads 0 */

@@ -115,3 +115,13 @@ def test_addresses_inside_an_element_are_refused(lib, dtype):
         for name, off in [(n, half) for n in tensors.split()] + [(n, 2) for n in words.split()]:
             assert entry(struct(**{**good, "dtype": dtype, name: FAKE + off}), None) == -1, name
             assert "aligned" in _lib.last_error(), (name, _lib.last_error())
+
+
+def test_more_heads_or_sequences_than_are_counted_are_refused(lib):
+    many = 1 << 30
+    assert lib.vafa_rotary(_lib.RotaryArgs(**{**_ROTARY, "num_heads": many, "num_kv_heads": many}), None) == -2 and "heads" in _lib.last_error()
+    assert lib.vafa_paged_append(_lib.PagedAppendArgs(**{**_APPEND, "num_kv_heads": many}), None) == -2 and "heads" in _lib.last_error()
+    for n in (many + 1, 2**31 - 1):
+        big = _lib.PagedAttnArgs(**{**_DECODE, "n_seq": n})
+        assert lib.vafa_paged_decode_workspace_bytes(big) == 0
+        assert lib.vafa_paged_decode(big, None) == -2 and "n_seq" in _lib.last_error()

@@ -21,6 +21,9 @@ int check_addresses(int dtype, std::initializer_list<const void*> tensors, std::
   return 0;
 }
 
+// Heads of a call of the rotation and the append, which count them in 32 bits.
+int check_heads(long long heads) { return heads > (1 << 30) ? fail(VAFA_ERR_UNSUPPORTED, "%lld heads", heads) : 0; }
+
 int check_table(const float* cos, const float* sin, int R, int D, int rows) {
   if (!cos || !sin) return fail(VAFA_ERR_INVALID, "null cos/sin");
   if (!aligned(cos, 4) || !aligned(sin, 4)) return fail(VAFA_ERR_INVALID, "cos/sin must be 4-byte aligned");
@@ -50,6 +53,7 @@ int check_decode(const vafa_paged_attn_args* a) {
   if (a->q_len < 1 || a->num_heads < 1 || a->num_kv_heads < 1 || a->num_heads % a->num_kv_heads)
     return fail(VAFA_ERR_INVALID, "bad sizes q_len=%d H=%d H_kv=%d (H_kv must divide H)", a->q_len, a->num_heads, a->num_kv_heads);
   if ((long long)a->q_len * a->num_heads > (1 << 18) || a->num_kv_heads > 0xffff) return fail(VAFA_ERR_UNSUPPORTED, "q_len %d x %d heads", a->q_len, a->num_heads);
+  if (a->n_seq > (1 << 30)) return fail(VAFA_ERR_UNSUPPORTED, "n_seq %d", a->n_seq);  // (a CTA's threads share out the sequences in 32 bits)
   return check_cache(a->n_seq, a->num_pages, a->page_size, a->max_pages);
 }
 
@@ -143,6 +147,7 @@ int vafa_rotary(const vafa_rotary_args* a, vafa_stream_t stream) {
   if (!a->positions && (!a->cu_seqlens || a->n_seg < 1)) return fail(VAFA_ERR_INVALID, "neither positions nor cu_seqlens");
   if (a->total > 0 && ((a->num_heads > 0 && (!a->q || !a->q_out)) || (a->num_kv_heads > 0 && (!a->k || !a->k_out))))
     return fail(VAFA_ERR_INVALID, "null q/k");
+  if (const int rc = check_heads((long long)a->num_heads + a->num_kv_heads)) return rc;
   if (const int rc = check_addresses(a->dtype, {a->q, a->k, a->q_out, a->k_out}, {a->positions, a->cu_seqlens, a->status})) return rc;
   return rotary_launch(a, (cudaStream_t)stream);
 }
@@ -162,6 +167,7 @@ int vafa_paged_append(const vafa_paged_append_args* a, vafa_stream_t stream) {
   if ((rc = check_cache(a->n_seq, a->num_pages, a->page_size, a->max_pages))) return rc;
   if (!a->cu_seqlens && a->total != a->n_seq) return fail(VAFA_ERR_INVALID, "without cu_seqlens total %d must be n_seq %d", a->total, a->n_seq);
   if (a->total > 0 && (!a->k || !a->v || (a->q && !a->q_out))) return fail(VAFA_ERR_INVALID, "null k/v/q_out");
+  if ((rc = check_heads((a->q ? a->num_heads : 0) + 2LL * a->num_kv_heads))) return rc;
   if ((rc = check_addresses(a->dtype, {a->q, a->k, a->v, a->q_out, a->k_cache, a->v_cache}, {a->cu_seqlens, a->cache_seqlens, a->page_table, a->status})))
     return rc;
   return paged_append_launch(a, (cudaStream_t)stream);
