@@ -63,6 +63,20 @@ def test_only_what_has_a_gradient_comes_back_with_one(monkeypatch, wants_q, want
     assert b is None and torch.equal(x.grad, torch.ones_like(x))
 
 
+def test_threads_that_make_the_status_word_at_once_get_the_same_one(monkeypatch):
+    monkeypatch.setattr(_lib, "_status", {})
+    dev, zeros, others = torch.device("cpu", 0), torch.zeros, []
+
+    def slow_zeros(*a, **kw):  # another thread comes in between
+        monkeypatch.setattr(torch, "zeros", zeros)
+        others.append(_lib.status_word(dev))
+        return zeros(*a, **kw)
+
+    monkeypatch.setattr(torch, "zeros", slow_zeros)
+    mine = _lib.status_word(dev)
+    assert others and mine is others[0] and _lib.status_word(dev) is mine
+
+
 def test_warps_whose_lanes_meet_again_give_up_together():
     """A wait that runs out is each lane's own verdict.  Where lanes shuffle, vote or wait for one another after it, it has to be one for all, or
     those that stay wait without a limit for those that left.  (Read from the source: no wait is made to run out.)"""

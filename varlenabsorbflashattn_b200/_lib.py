@@ -176,7 +176,7 @@ def status_word(device: torch.device) -> torch.Tensor:
     if t is None:
         with torch.inference_mode(False):  # (made by a first call under inference mode it could not be cleared outside)
             t = torch.zeros(STATUS_WORDS, dtype=torch.int32, device=device)
-        _status[key] = t
+        t = _status.setdefault(key, t)  # (another thread may have been first: one word for all of them)
     return t
 
 
