@@ -1,14 +1,14 @@
-"""Rotation, paged append and paged decode on the GPU: arguments of other types and kinds than the usual ones."""
+"""Rotation, paged append and paged decode on the GPU: arguments of other types, kinds and sizes than the usual ones."""
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 import varlenabsorbflashattn_b200 as vb
 from varlenabsorbflashattn_b200 import _lib
-from paged_ref import paged_cache
+from paged_ref import assert_within, decode, paged_cache, positions_of, rotate, rotation_error
 
 pytestmark = pytest.mark.gpu
-BF16, F32 = torch.bfloat16, torch.float32
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
 
 
 @pytest.fixture
@@ -134,3 +134,57 @@ def test_autograd_is_told_of_either_cache(kept):
     vb.paged_kv_append(k, k, caches["k"], caches["v"], page_table=table, cache_seqlens=_ints([8, 8]))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+@pytest.mark.parametrize("dtype,H,H_kv,D,R", [(F32, 32, 8, 128, 128), (F32, 80, 8, 128, 64), (BF16, 88, 88, 128, 128), (F16, 60, 30, 256, 2), (F32, 40, 8, 256, 256)])
+def test_long_batches_of_wide_tokens(dtype, H, H_kv, D, R):
+    """Token rows of more than half a tile of shared memory (one token a tile), up to those that do not fit four times (48 KB)."""
+    gen = _gen(H)
+    T = (11 << 20) // ((H + H_kv) * D * dtype.itemsize) + 3
+    lens = [1, 0, 100, T - 101]
+    qkv = _randn(gen, T, H + 2 * H_kv, D, dtype=dtype)
+    q, k, v = qkv[:, :H], qkv[:, H:H + H_kv], qkv[:, H + H_kv:]
+    cos, sin = vb.rotary_table(max(lens), R, device="cuda")
+    pos = positions_of(lens).cuda()
+    out = vb.packed_rotary(q, k, cos, sin, cu_seqlens=_cu(lens))
+    for name, x, y in zip("qk", (q, k), out):
+        ref, mag = rotate(x, cos, sin, pos, False)
+        assert_within(y, ref, rotation_error(ref, mag, dtype), name)
+    kc, vc, table = paged_cache(lens, H_kv, D, 16, dtype, gen, fill=7.0)
+    want = kc.clone(), vc.clone()
+    at = table[torch.repeat_interleave(torch.arange(4), torch.tensor(lens)).cuda(), pos // 16].long(), pos % 16
+    want[0][at], want[1][at] = out[1], v
+    got = vb.paged_kv_append(k, v, kc, vc, page_table=table, cache_seqlens=_ints(lens), cu_seqlens=_cu(lens), q=q, cos=cos, sin=sin)
+    assert torch.equal(got, out[0]) and torch.equal(kc, want[0]) and torch.equal(vc, want[1])
+
+
+@pytest.mark.parametrize("dtype,D", [(BF16, 64), (F16, 16), (F32, 32)])
+@pytest.mark.parametrize("T", [1, 4000])
+def test_append_to_caches_at_any_address(dtype, D, T):
+    """Caches with an odd offset and an odd pitch of pages, slots and heads: only the elements of the new tokens change."""
+    gen, H_kv, page = _gen(T), 8, 24
+    pages = -(-T // page) + 2
+    whole = [torch.full((pages, page + 1, H_kv + 1, D + 3), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+    kc, vc = (x[:, 1:, 1:, 3:] for x in whole)
+    assert kc.data_ptr() % 16 and kc.stride(2) % 2
+    table = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32)[None]
+    k, v = (_randn(gen, T, H_kv, D, dtype=dtype) for _ in range(2))
+    pos = torch.arange(T, device="cuda")
+    want = [x.clone() for x in whole]
+    for w, x in zip(want, (k, v)):
+        w[:, 1:, 1:, 3:][table[0, pos // page].long(), pos % page] = x
+    vb.paged_kv_append(k, v, kc, vc, page_table=table, cache_seqlens=_ints([T]), cu_seqlens=_cu([T]))
+    assert all(torch.equal(a, b) for a, b in zip(whole, want))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_lse_of_equal_weights(dtype):
+    """scale 0: o is the mean of the values, lse the logarithm of their number."""
+    gen, lens, H, H_kv, D = _gen(6), [40, 3, 200, 0, 5000], 6, 3, 64
+    kc, vc, table = paged_cache(lens, H_kv, D, 8, dtype, gen)
+    q = _randn(gen, len(lens), 2, H, D, dtype=dtype)
+    o, lse = vb.paged_decode_attn_with_lse(q, kc, vc, page_table=table, cache_seqlens=_ints(lens), scale=0.0)
+    ro, rl, eo, el = decode(q, kc, vc, table, lens, scale=0.0)
+    assert_within(o, ro, eo, "o")
+    assert_within(lse, rl, el, "lse")
+    assert (lse[3] == -float("inf")).all() and abs(lse[4, 1, 0].item() - torch.tensor(5000.0).log().item()) < 1e-5
