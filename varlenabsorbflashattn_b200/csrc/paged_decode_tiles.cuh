@@ -12,11 +12,9 @@
 // 16-bit P is split into two pieces (hi + lo) for the second product: one piece would put an error of the size of the output's own
 // rounding on top of it (2.4e-3 instead of 1.7e-3 of bf16 outputs); the second costs a product per V fragment and no time that shows.
 // fp16 P is held larger than it is, for its short range (kLift).
-// Where V is not finite (looked for in every fragment) its keys are summed apart, by multiply-adds with whole weights, for the rows that see them:
-// 0 times a NaN would reach the rows that do not see it (the new tokens themselves), and the two pieces of P give inf - inf
-// or 0 inf where the weight itself gives inf.  The look costs an instruction a register of V: nothing up to 16 rows, us without | with
-// it on 64 caches of 4k to 8k keys, heads of 128: four tokens of 8 grouped heads 335 | 341, seven 516 | 567 (shared out among the row groups with a
-// barrier behind it 363 and 555).
+// Keys that some rows see and others do not (the new tokens themselves) are summed apart where V is not finite: 0 times a
+// NaN would reach the rows that do not see it.  An infinite V that a row sees may come out of the two pieces of P as inf - inf or 0 inf;
+// such a sum is NaN, and once the warps are joined its infinite addends decide it (bad_values in paged_decode.cuh).
 #pragma once
 #include <type_traits>
 
@@ -82,14 +80,6 @@ template <typename T>
 __device__ __forceinline__ bool not_finite2(uint32_t x) {
   constexpr uint32_t e = sizeof(T) == 2 && std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
   return (x & e) == e || (x & (e << 16)) == (e << 16);
-}
-// The larger magnitudes of two pairs, NaN where one is (signs as they come).
-template <typename T>
-__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  if constexpr (std::is_same<T, __half>::value) asm("max.NaN.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  else asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -273,24 +263,40 @@ struct NarrowTile {
         pl[e] = transpose8(pl[e]);
       }
       const int first = b.first + key0 + 16 * t;
+      const int apart0 = p.T > 1 && b.masked ? max(0, b.every - first) : 16;
+      const int apart1 = min(16, b.len - first);
 #pragma unroll
       for (int d0 = 0; d0 < D / 16; d0 += kAhead) {
         if (t > 0 || d0 > 0) {
 #pragma unroll
           for (int d = 0; d < kAhead; ++d) ldsm4t(va[d], vs + t * 16 * C::PITCH + (((2 * (d0 + d) + ((lane >> 3) & 1)) ^ v_key) << 4));
         }
-        uint32_t largest = 0;
+        bool apart = false;
+        if (apart0 < apart1) {
 #pragma unroll
-        for (int d = 0; d < kAhead; ++d)
+          for (int d = 0; d < kAhead; ++d)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) largest = max_abs2<T>(largest, va[d][x]);
-        if (!__any_sync(0xffffffffu, not_finite2<T>(largest))) {
+            for (int x = 0; x < 4; ++x) apart |= not_finite2<T>(va[d][x]);
+          apart = __any_sync(0xffffffffu, apart);
+        }
+        if (apart) {  // V without those keys: a register holds the lane's pair of keys, or the pair 8 on
+          const int a0 = 2 * (lane & 3);
+          const uint32_t keep0 = (a0 < apart0 ? 0xffffu : 0u) | (a0 + 1 < apart0 ? 0xffff0000u : 0u);
+          const uint32_t keep1 = (a0 + 8 < apart0 ? 0xffffu : 0u) | (a0 + 9 < apart0 ? 0xffff0000u : 0u);
 #pragma unroll
-          for (int d = 0; d < kAhead; ++d) mma<T>(o[d0 + d], va[d], ph[0], ph[1]);
+          for (int d = 0; d < kAhead; ++d) {
+            va[d][0] &= keep0;
+            va[d][1] &= keep0;
+            va[d][2] &= keep1;
+            va[d][3] &= keep1;
+          }
+        }
 #pragma unroll
-          for (int d = 0; d < kAhead; ++d) mma<T>(o[d0 + d], va[d], pl[0], pl[1]);
-        } else {
-          for (int k = 0; k < min(16, b.len - first); ++k) {
+        for (int d = 0; d < kAhead; ++d) mma<T>(o[d0 + d], va[d], ph[0], ph[1]);
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) mma<T>(o[d0 + d], va[d], pl[0], pl[1]);
+        if (apart) {
+          for (int k = apart0; k < apart1; ++k) {
             const unsigned char* const row = b.v + (key0 + 16 * t + k) * C::PITCH;
             const int ck = C::key(key0 + 16 * t + k);
             auto v_at = [&](int ch) { return to_float(reinterpret_cast<const T*>(row + (ch ^ ck) * 16)[lane >> 2]); };  // head dim 8 ch + lane / 4
@@ -472,28 +478,44 @@ struct WideTile {
 #pragma unroll
         for (int x = 0; x < 2; ++x) split2<T>(s[2 * t + e][2 * x], s[2 * t + e][2 * x + 1], ph[2 * e + x], pl[2 * e + x]);
       const int first = b.first + key0 + 16 * t;
+      const int apart0 = p.T > 1 && b.masked ? max(0, b.every - first) : 16;
+      const int apart1 = min(16, b.len - first);
 #pragma unroll
       for (int d0 = 0; d0 < D / 16; d0 += kAheadV) {
         if (t > 0 || d0 > 0) {
 #pragma unroll
           for (int d = 0; d < kAheadV; ++d) ldsm4t(va[d], vs + t * 16 * C::PITCH + (((2 * (d0 + d) + (lane >> 4)) ^ v_key) << 4));
         }
-        uint32_t largest = 0;
+        bool apart = false;
+        if (apart0 < apart1) {
+#pragma unroll
+          for (int d = 0; d < kAheadV; ++d)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) apart |= not_finite2<T>(va[d][x]);
+          apart = __any_sync(0xffffffffu, apart);
+        }
+        if (apart) {  // V without those keys: a register holds the lane's pair of keys, or the pair 8 on
+          const int a0 = 2 * (lane & 3);
+          const uint32_t keep0 = (a0 < apart0 ? 0xffffu : 0u) | (a0 + 1 < apart0 ? 0xffff0000u : 0u);
+          const uint32_t keep1 = (a0 + 8 < apart0 ? 0xffffu : 0u) | (a0 + 9 < apart0 ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int d = 0; d < kAheadV; ++d) {
+            va[d][0] &= keep0;
+            va[d][1] &= keep1;
+            va[d][2] &= keep0;
+            va[d][3] &= keep1;
+          }
+        }
 #pragma unroll
         for (int d = 0; d < kAheadV; ++d)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) largest = max_abs2<T>(largest, va[d][x]);
-        if (!__any_sync(0xffffffffu, not_finite2<T>(largest))) {
+          for (int e = 0; e < 2; ++e) mma<T>(o[2 * (d0 + d) + e], ph, va[d][2 * e], va[d][2 * e + 1]);
 #pragma unroll
-          for (int d = 0; d < kAheadV; ++d)
+        for (int d = 0; d < kAheadV; ++d)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) mma<T>(o[2 * (d0 + d) + e], ph, va[d][2 * e], va[d][2 * e + 1]);
-#pragma unroll
-          for (int d = 0; d < kAheadV; ++d)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) mma<T>(o[2 * (d0 + d) + e], pl, va[d][2 * e], va[d][2 * e + 1]);
-        } else {
-          for (int k = 0; k < min(16, b.len - first); ++k) {
+          for (int e = 0; e < 2; ++e) mma<T>(o[2 * (d0 + d) + e], pl, va[d][2 * e], va[d][2 * e + 1]);
+        if (apart) {
+          for (int k = apart0; k < apart1; ++k) {
             const unsigned char* const row = b.v + (key0 + 16 * t + k) * C::PITCH;
             const int ck = C::key(key0 + 16 * t + k);
             const int src = (lane & 28) | ((k & 7) >> 1);
