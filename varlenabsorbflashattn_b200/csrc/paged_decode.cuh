@@ -605,9 +605,9 @@ Plan plan_of(int R) { return Plan{C::ROWS, (R + C::ROWS - 1) / C::ROWS, C::CTAS,
 // often an SM reads a block from shared memory.  64 caches of 4k to 8k keys with 8 K/V heads of 128, us:
 //   up to 8 rows     narrow; 1 | 2 | 3 CTAs an SM (128 caches of 8k to 32k keys) 2782 | 1585 | 1427
 //   up to 16         wide, 4 warps on a block, 3 CTAs: 256; two 264, one 442; two warps on a block 351; narrow with two column tiles 292
-//   up to 32         wide, 2 row groups of 2 warps, 2 CTAs: 333; (of the first version) 361; one CTA 592; 4 warps a group 441, one 532
-//   up to 64         wide, 4 row groups of 1 warp, 2 CTAs: 515; (of the first version) 534; of 2 warps, one CTA 636; of 4 warps 1165
-//   heads of 256     O takes twice the registers: narrow with two row groups to 16 rows, 284 (wide 376), wide beyond
+//   up to 32         wide, 2 row groups of 2 warps, 2 CTAs: 345; (of the first version) 361; one CTA 592; 4 warps a group 441, one 532
+//   up to 64         wide, 4 row groups of 1 warp, 2 CTAs: 531; (of the first version) 534; of 2 warps, one CTA 636; of 4 warps 1165
+//   heads of 256     O takes twice the registers: narrow with two row groups to 16 rows, 284 (wide 376), wide beyond (28 rows 387)
 //   fp32             4 rows a warp where units have no more, 3 CTAs: 507; 8 rows 877 (two groups of 4: 851, but no gain with more rows)
 template <typename T, int D>
 Plan plan_for(int R) {
@@ -616,7 +616,7 @@ Plan plan_for(int R) {
     if (R <= 8) return plan_of<Config<T, D, kFma8, 1, 4, 3>>(R);
     return plan_of<Config<T, D, kFma8, 2, 4, 2>>(R);
   } else {
-    if (R <= 8) return plan_of<Config<T, D, kNarrow, 1, 4, D == 256 ? 2 : 3>>(R);
+    if (R <= 8) return plan_of<Config<T, D, kNarrow, 1, 4, 3>>(R);  // (one CTA at heads of 256: no room for two)
     if constexpr (D == 256) {
       if (R <= 16) return plan_of<Config<T, D, kNarrow, 2, 4, 1>>(R);
       return plan_of<Config<T, D, kWide, 2, 4, 1>>(R);

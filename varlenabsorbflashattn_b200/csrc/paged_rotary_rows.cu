@@ -2,8 +2,8 @@
 //
 // The work per byte is a few instructions, so what counts is how many bytes are on their way.  Held in registers (paged_rotary.cu)
 // they are 30 to 60 KB an SM, and a block's start, look-ups and loads follow one another: 4.1 TB/s.  Here a warp looks positions
-// and places up and sends for the rows and angles of a tile of tokens by bulk copies, up to eight tiles ahead; sixteen warps rotate them in
-// place in shared memory, in groups that take turns; another warp sends them to the outputs, or to the cache's slots, by bulk
+// and places up and sends for the rows and angles of a tile of tokens by bulk copies, four tiles ahead (eight, where 216 KB hold as many: 27 KB
+// or less); sixteen warps rotate them in place in shared memory, in groups that take turns; another warp sends them to the outputs, or to the cache's slots, by bulk
 // copies.  Values that only move (v) are not touched by a thread.  151 k tokens of 40 heads of 128 (3.1 GB in and out): 0.49 ms,
 // 6.3 TB/s, 96 % of a plain copy; into a cache of pages of 16 (18 k tokens, 0.45 GB) 75 us, 91 %.
 #include <atomic>

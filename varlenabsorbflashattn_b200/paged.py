@@ -23,7 +23,8 @@ once validation is off, with lengths and tables that change in place between rep
 As in `packed_varlen_attn` all arithmetic happens in libvafa_b200.so.  With validation on (`set_validate_cu_seqlens`,
 the default) lengths, page ids and positions are checked on the host, which waits for the device; a serving loop
 switches it off.  Unchecked, an index that leaves its array is not followed on the device either: nothing outside the tensors is read or
-written, and the status word reports it (`_lib.check_status`).
+written, and the status word reports it (`_lib.check_status`).  Lengths, tables, positions and prefix sums are taken from any integer type and device;
+int32 on the device of the rest, in tensors of three dims (four for a decode of several tokens), is the fast way: other ones are converted in each call.
 """
 from __future__ import annotations
 
