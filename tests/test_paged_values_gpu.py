@@ -105,3 +105,26 @@ def test_infinite_values_that_a_row_sees(dtype, D, H, H_kv, T):
     o, lse = vb.paged_decode_attn_with_lse(q, kc, vc, page_table=table, cache_seqlens=_ints(lens))
     assert_within(lse, rl, el, "lse")
     assert_within(o, ro, eo, "o")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("D,H,H_kv,T", [(64, 4, 2, 1), (128, 4, 1, 4), (256, 8, 1, 1), (32, 16, 1, 4)])
+def test_values_that_are_nan_or_of_every_kind(dtype, D, H, H_kv, T):
+    """NaN in one place, in a whole head dim, everywhere; infinite values in every key; each beside dims that are finite."""
+    gen, lens, inf, nan = _gen(D + 1), [700, 700, 700, 700], float("inf"), float("nan")
+    kc, vc, table = paged_cache(lens, H_kv, D, 16, dtype, gen)
+    q = _randn(gen, len(lens), T, H, D, dtype=dtype)
+    pages = [table[i, :44].long() for i in range(4)]
+    vc[pages[0][20], 3, :, 5] = nan
+    vc[pages[0][40], 1, :, 5] = inf
+    vc[pages[0][40], 2, :, 4] = -inf
+    vc[pages[1], :, :, 7] = nan
+    vc[pages[1], :, :, 9] = inf
+    vc[pages[2], :, :, D // 2:] = -inf
+    vc[pages[2][0], 0, :, D - 1] = inf
+    vc[pages[3]] = nan
+    ro, rl, eo, el = decode(q, kc, vc, table, lens)
+    o, lse = vb.paged_decode_attn_with_lse(q, kc, vc, page_table=table, cache_seqlens=_ints(lens))
+    assert o[3].isnan().all() and o[0, ..., 5].isnan().all() and (o[0, ..., 4] == -inf).all() and (o[1, ..., 9] == inf).all()
+    assert_within(lse, rl, el, "lse")
+    assert_within(o, ro, eo, "o")

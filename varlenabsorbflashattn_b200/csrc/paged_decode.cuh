@@ -166,40 +166,45 @@ struct Block {  // a block of the line, as its ring slot describes it
 // Four dims of a row's sum of p v where P went into the product as two pieces and the sum is NaN although the weights are numbers: an infinite
 // value gave inf - inf, or 0 inf where a piece is zero.  The values of keys [from, to) that are not finite decide, each with its whole
 // weight, and where there is none NaN stays.  (64 caches of 4k to 8k keys, heads of 128, seven tokens of 8 grouped heads: 516 us without, 531 with
-// this, 567 with a look over every block's values before the product; up to 16 rows level.)
+// this, 567 with a look over every block's values before the product; up to 16 rows level.  A thread walks over its keys until nothing
+// more can change: 64 caches of 16k keys, 8 heads, whose last key alone is infinite or NaN in all dims 12 ms instead of 0.65, NaN everywhere 0.65.)
 template <typename T, int D, typename Read, typename Write>
 __device__ __forceinline__ void bad_values(const DecodeParams& p, int seq, int h, int r, int from, int to, int d, float m, Read sum, Write set) {
   const int t = r / p.g;
   const T* const q = reinterpret_cast<const T*>(p.q) + seq * p.q_seq + t * p.q_token + (h * p.g + r - t * p.g) * p.q_head;
   float now[4] = {0.f, 0.f, 0.f, 0.f};
-  int found = 0, asked = 0;
+  int found = 0, open = 0;  // dims that a value has been found for, dims that another one could change
 #pragma unroll
-  for (int x = 0; x < 4; ++x) asked |= isnan(sum(x)) << x;
-  if (asked == 0) return;
+  for (int x = 0; x < 4; ++x) open |= isnan(sum(x)) << x;
 #pragma unroll 1
-  for (int j = from; j < to; ++j) {
+  for (int j = from; j < to && open; ++j) {
     const int row = page_of(p, j), page = p.table[seq * p.table_stride + row], slot = j - row * p.page_size;
     if (page < 0 || page >= p.num_pages) continue;
     const T* const v = reinterpret_cast<const T*>(p.v) + page * p.v_page + slot * p.v_slot + h * p.v_head + d;
     const uint2 raw = *reinterpret_cast<const uint2*>(v);
     if (!not_finite2<T>(raw.x) && !not_finite2<T>(raw.y)) continue;
-    const T* const k = reinterpret_cast<const T*>(p.k) + page * p.k_page + slot * p.k_slot + h * p.k_head;
-    float s = 0.f;
-#pragma unroll 1
-    for (int i = 0; i < D; ++i) s = fmaf(to_float(q[i]), to_float(k[i]), s);
-    const float w = exp2_approx(s * p.scale_log2 - m);
+    float w = 0.f;
+    bool known = false;
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const float value = to_float(v[x]);
-      if (!isfinite(value)) {
-        now[x] = fmaf(w, value, now[x]);
-        found |= 1 << x;
+      if (isfinite(value) || !(open >> x & 1)) continue;
+      if (!isnan(value) && !known) {
+        const T* const k = reinterpret_cast<const T*>(p.k) + page * p.k_page + slot * p.k_slot + h * p.k_head;
+        float s = 0.f;
+#pragma unroll 8
+        for (int i = 0; i < D; ++i) s = fmaf(to_float(q[i]), to_float(k[i]), s);
+        w = exp2_approx(s * p.scale_log2 - m);
+        known = true;
       }
+      now[x] = fmaf(w, value, now[x]);  // (NaN whatever the weight)
+      found |= 1 << x;
+      if (isnan(now[x])) open &= ~(1 << x);
     }
   }
 #pragma unroll
   for (int x = 0; x < 4; ++x)
-    if (asked & found & (1 << x)) set(x, now[x]);
+    if (found >> x & 1) set(x, now[x]);
 }
 
 template <typename C>
@@ -607,7 +612,7 @@ Plan plan_of(int R) { return Plan{C::ROWS, (R + C::ROWS - 1) / C::ROWS, C::CTAS,
 //   up to 16         wide, 4 warps on a block, 3 CTAs: 256; two 264, one 442; two warps on a block 351; narrow with two column tiles 292
 //   up to 32         wide, 2 row groups of 2 warps, 2 CTAs: 345; (of the first version) 361; one CTA 592; 4 warps a group 441, one 532
 //   up to 64         wide, 4 row groups of 1 warp, 2 CTAs: 531; (of the first version) 534; of 2 warps, one CTA 636; of 4 warps 1165
-//   heads of 256     O takes twice the registers: narrow with two row groups to 16 rows, 284 (wide 376), wide beyond (28 rows 387)
+//   heads of 256     O takes twice the registers: narrow with two row groups to 16 rows, 287 (wide 376), wide beyond (28 rows 387)
 //   fp32             4 rows a warp where units have no more, 3 CTAs: 507; 8 rows 877 (two groups of 4: 851, but no gain with more rows)
 template <typename T, int D>
 Plan plan_for(int R) {
